@@ -1,7 +1,8 @@
 /*
  * picotron_b200.h -- C ABI of the B200 (sm_100a) RMSNorm / SwiGLU / RoPE hot path and the
  * next-step kernels around it (fused residual add + RMSNorm, SwiGLU fused into the gate/up
- * GEMM, cross-entropy, AdamW).
+ * GEMM, cross-entropy, AdamW) and of post-training (token log-probabilities, preference and
+ * policy losses, AdamW with 8-bit states, RoPE by positions).
  *
  * This is the drop-in boundary for picotron's `model.triton_kernels.{rmsnorm,swiglu,rope}`
  * kernels. Every entry point takes plain device pointers, element counts, strides (in
@@ -270,8 +271,8 @@ PT_API int pt_add_rmsnorm_bwd_fused(const void* dy, int64_t dy_row_stride,
  * (synchronous: waits for the device). *code = 0 means no kernel reported a problem;
  * 1 means a kernel gave up waiting for one of its own TMA copies or MMAs (after about a
  * second) and skipped the rest of its work, so outputs of the affected call are incomplete;
- * 2 means pt_cross_entropy_fwd met a target outside [0, vocab) that is not ignore_index
- * (its row loss, and so the mean, is NaN).
+ * 2 means pt_cross_entropy_fwd or a logit loss met a target outside [0, vocab) that is not
+ * ignore_index (its row loss or log-probability, and so the loss, is NaN).
  * No reference counterpart: the reference has no device-side waits. */
 PT_API int pt_take_device_error(int* code);
 
@@ -379,6 +380,83 @@ PT_API int pt_cross_entropy_bwd(const void* logits, int64_t vocab, int64_t outer
                                 int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
                                 int dtype, void* stream);
 
+/* --------------------------------------- log-probabilities, post-training losses -- */
+
+/* The logit losses read rows of `vocab` logits as pt_cross_entropy_fwd does: an [outer, inner]
+ * grid (sequences x positions) with two row strides in elements, class stride 1, an int64
+ * target per row with its own two strides, f32 / f16 / bf16 logits, fp32 math. Rows whose
+ * target is ignore_index are not read: they have no log-probability (0 is written), no part in
+ * any loss and a gradient of zeros, whatever their logits and per-token inputs hold. A target
+ * outside [0, vocab) gives NaN and sets the device error word; its gradient is zeros. A row
+ * with no finite logit gives NaN. Per-token inputs are fp32 with two strides each (0 broadcasts).
+ * The reference's post-training package (src/picotron_sft, src/picotron_dpo) evaluates such
+ * losses in PyTorch; these entry points have no kernel counterpart there.
+ *
+ * Bytes of device workspace (16-byte aligned, caller-owned, nothing kept between calls) that the
+ * forward of a problem needs on the current device. */
+PT_API int pt_logit_loss_workspace(int64_t vocab, int64_t outer, int64_t inner, int dtype,
+                                   int64_t* bytes);
+
+/* logps[r] = x_r[target] - log(sum(exp(x_r))) (dense [rows]) and stats[r] = (max(x_r), 1 /
+ * sum(exp(x_r - max))) (dense [rows, 2]), which the backward reads. */
+PT_API int pt_token_logps_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                              int64_t logits_outer_stride, int64_t logits_inner_stride,
+                              const int64_t* targets, int64_t targets_outer_stride,
+                              int64_t targets_inner_stride, int64_t ignore_index, float* logps,
+                              float* stats, void* workspace, int64_t workspace_size, int dtype,
+                              void* stream);
+
+/* dlogits[r] = c_r (onehot(target_r) - softmax(x_r)), c_r = coef[r] * grad (coef: the loss's
+ * derivative to logps, with two strides; grad: one fp32 value in device memory, or NULL for 1).
+ * The backward of all the losses here, from the stats and coef of their forward. Rows of dlogits
+ * must have the same address modulo 16 bytes as those of logits, and not overlap them. */
+PT_API int pt_token_logps_bwd(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                              int64_t logits_outer_stride, int64_t logits_inner_stride,
+                              const int64_t* targets, int64_t targets_outer_stride,
+                              int64_t targets_inner_stride, int64_t ignore_index,
+                              const float* stats, const float* coef, int64_t coef_outer_stride,
+                              int64_t coef_inner_stride, const float* grad, void* dlogits,
+                              int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
+                              int dtype, void* stream);
+
+/* Preference loss of pairs: sequences 0 .. outer/2 - 1 are the chosen answers, the rest the
+ * rejected ones in the same order. With rewards[q] = beta * sum over q's positions with a target
+ * of (logp - reference) and z = rewards[chosen] - rewards[rejected]:
+ *   loss = mean over pairs of (1 - label_smoothing) softplus(-z) + label_smoothing softplus(z).
+ * reference: the frozen model's log-probability of each target. The sums are taken in 64 bits.
+ * Writes loss (one value; NaN for no pairs), rewards [outer], stats [rows, 2] and
+ * coef [outer] = d loss / d logp of every position of a sequence (strides (1, 0) for
+ * pt_token_logps_bwd). */
+PT_API int pt_preference_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                                  int64_t logits_outer_stride, int64_t logits_inner_stride,
+                                  const int64_t* targets, int64_t targets_outer_stride,
+                                  int64_t targets_inner_stride, int64_t ignore_index,
+                                  const float* reference, int64_t reference_outer_stride,
+                                  int64_t reference_inner_stride, double beta,
+                                  double label_smoothing, float* loss, float* rewards,
+                                  float* stats, float* coef, void* workspace,
+                                  int64_t workspace_size, int dtype, void* stream);
+
+/* Clipped policy loss: with r = exp(logp - old_logps), A = advantages and g = reference - logp,
+ * each position with a target costs
+ *   max(-A r, -A min(max(r, 1 - clip_low), 1 + clip_high)) + kl_coef (exp(g) - g - 1),
+ * without the second term when reference is NULL. The loss is the mean over all such positions
+ * (by_sequence = 0) or the mean over sequences that have any of their means (by_sequence = 1);
+ * NaN when there are none. Writes loss, logps [rows], stats [rows, 2] and coef [rows] (for
+ * pt_token_logps_bwd); the gradient takes the unclipped branch where both are equal. */
+PT_API int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                              int64_t logits_outer_stride, int64_t logits_inner_stride,
+                              const int64_t* targets, int64_t targets_outer_stride,
+                              int64_t targets_inner_stride, int64_t ignore_index,
+                              const float* old_logps, int64_t old_outer_stride,
+                              int64_t old_inner_stride, const float* advantages,
+                              int64_t advantages_outer_stride, int64_t advantages_inner_stride,
+                              const float* reference, int64_t reference_outer_stride,
+                              int64_t reference_inner_stride, double clip_low, double clip_high,
+                              double kl_coef, int by_sequence, float* loss, float* logps,
+                              float* stats, float* coef, void* workspace, int64_t workspace_size,
+                              int dtype, void* stream);
+
 /* ------------------------------------------------------------------ AdamW -------- */
 
 /* One fused AdamW step over num_tensors fp32 parameters (device pointers in host arrays):
@@ -396,6 +474,34 @@ PT_API int pt_adamw_step(float* const* params, const float* const* grads,
                          const int64_t* numels, const int64_t* steps, const double* lrs,
                          const double* weight_decays, int num_tensors, double beta1,
                          double beta2, double eps, int maximize, void* stream);
+
+/* One AdamW step over num_tensors parameters (dtype f32, f16 or bf16, gradients of the same)
+ * whose moments are held in 8 bits, in blocks of 256 consecutive elements with one fp32 scale a
+ * block (the last block may be short):
+ *   exp_avg = c |c| scale, c the int8 code (|c| <= 127);  exp_avg_sq = c^4 scale, c the uint8 code.
+ * The update is pt_adamw_step's formula in fp32; new moments are m = b1 m + (1 - b1) g and
+ * v = b2 v + (1 - b2) (g g) with each product and sum rounded to fp32, new scales max|m| / 127^2
+ * and max v / 255^4 of the block (0 where that is below the smallest normal number), new codes
+ * the nearest ones in the square-root / fourth-root domain (ties to even), at least 1 where
+ * v > 0. Code arrays have numels[i] elements, scale arrays ceil(numels[i] / 256); zeros are the
+ * state before the first step. The parameters must not overlap one another. A non-finite
+ * gradient makes the moments of its whole block non-finite. No reference counterpart (its
+ * optimizer is torch.optim.AdamW, src/picotron/training/train_loop.py:302-325). */
+PT_API int pt_adamw8_step(void* const* params, const void* const* grads,
+                          int8_t* const* exp_avg_codes, float* const* exp_avg_scales,
+                          uint8_t* const* exp_avg_sq_codes, float* const* exp_avg_sq_scales,
+                          const int64_t* numels, const int64_t* steps, const double* lrs,
+                          const double* weight_decays, int num_tensors, double beta1,
+                          double beta2, double eps, int maximize, int dtype, void* stream);
+
+/* The fp32 moments that 8-bit states stand for: exp_avgs[i] and exp_avg_sqs[i], numels[i]
+ * elements each, from the arrays of pt_adamw8_step. No reference counterpart. */
+PT_API int pt_adamw8_moments(const int8_t* const* exp_avg_codes,
+                             const float* const* exp_avg_scales,
+                             const uint8_t* const* exp_avg_sq_codes,
+                             const float* const* exp_avg_sq_scales, const int64_t* numels,
+                             float* const* exp_avgs, float* const* exp_avg_sqs, int num_tensors,
+                             void* stream);
 
 /* ------------------------------------------------------------------- RoPE -------- */
 
@@ -439,6 +545,24 @@ PT_API int pt_rope_qk_bwd(const void* dq, const int64_t dq_strides[4], void* dq_
                           const int64_t dk_out_strides[4], const int64_t k_sizes[4],
                           const void* cosine, const void* sine, int64_t table_row_stride,
                           int layout, int dtype, int table_dtype, void* stream);
+
+/* Rotary embedding of a query and a key [B, H, S, D] (sizes and strides as above; the two share
+ * B, S and D) by explicit positions: token (b, s) turns pair i by the angle
+ * positions[b * position_batch_stride + s * position_stride] * inv_freq[i], evaluated in 64
+ * bits (positions may be far, negative, and in any order), with cosine and sine multiplied by
+ * `scale` (the attention scale of a long-context method; 1 otherwise). inv_freq holds
+ * rotary_dim / 2 fp64 frequencies. Only the first rotary_dim elements of a head are rotated,
+ * in pairs (x[2i], x[2i+1]) or (x[i], x[i + rotary_dim/2]) by `layout`; the rest is copied.
+ * backward = 1 applies the transpose (dq, dk in the place of q, k). One rounding per output;
+ * outputs do not overlap inputs. Extends RotaryEmbedding.forward (src/picotron/nn/rope.py:
+ * 70-107), whose positions are always 0 .. S-1. */
+PT_API int pt_rope_positions(const void* q, const int64_t q_strides[4], void* q_out,
+                             const int64_t q_out_strides[4], const int64_t q_sizes[4],
+                             const void* k, const int64_t k_strides[4], void* k_out,
+                             const int64_t k_out_strides[4], const int64_t k_sizes[4],
+                             const int64_t* positions, int64_t position_batch_stride,
+                             int64_t position_stride, const double* inv_freq, int64_t rotary_dim,
+                             double scale, int backward, int layout, int dtype, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

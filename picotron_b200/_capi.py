@@ -48,6 +48,11 @@ _c_int = ctypes.c_int
 _c_float = ctypes.c_float
 _c_ptr = ctypes.c_void_p
 _c_i64_4 = ctypes.c_int64 * 4
+_c_ptrs = ctypes.POINTER(ctypes.c_void_p)
+
+# Argument groups of the logit losses: a pointer with two row strides; logits and targets.
+_ROWS = [_c_ptr, _c_i64, _c_i64]
+_LOGITS = [_c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, *_ROWS, _c_i64]
 
 # name -> (restype, argtypes). Mirrors include/picotron_b200.h one to one; the CPU test
 # suite checks that every function declared there is exported and listed here.
@@ -100,6 +105,27 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pt_rope_qk_bwd": (_c_int, [_c_ptr, _c_i64_4, _c_ptr, _c_i64_4, _c_i64_4, _c_ptr, _c_i64_4,
                                 _c_ptr, _c_i64_4, _c_i64_4, _c_ptr, _c_ptr, _c_i64, _c_int,
                                 _c_int, _c_int, _c_ptr]),
+    "pt_rope_positions": (_c_int, [_c_ptr, _c_i64_4, _c_ptr, _c_i64_4, _c_i64_4, _c_ptr,
+                                   _c_i64_4, _c_ptr, _c_i64_4, _c_i64_4, _c_ptr, _c_i64, _c_i64,
+                                   _c_ptr, _c_i64, ctypes.c_double, _c_int, _c_int, _c_int,
+                                   _c_ptr]),
+    "pt_logit_loss_workspace": (_c_int, [_c_i64, _c_i64, _c_i64, _c_int,
+                                         ctypes.POINTER(_c_i64)]),
+    "pt_token_logps_fwd": (_c_int, [*_LOGITS, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
+    "pt_token_logps_bwd": (_c_int, [*_LOGITS, _c_ptr, *_ROWS, _c_ptr, *_ROWS, _c_int, _c_ptr]),
+    "pt_preference_loss_fwd": (_c_int, [*_LOGITS, *_ROWS, ctypes.c_double, ctypes.c_double,
+                                        _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int,
+                                        _c_ptr]),
+    "pt_policy_loss_fwd": (_c_int, [*_LOGITS, *_ROWS, *_ROWS, *_ROWS, ctypes.c_double,
+                                    ctypes.c_double, ctypes.c_double, _c_int, _c_ptr, _c_ptr,
+                                    _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
+    "pt_adamw8_step": (_c_int, [_c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs,
+                                ctypes.POINTER(_c_i64), ctypes.POINTER(_c_i64),
+                                ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),
+                                _c_int, ctypes.c_double, ctypes.c_double, ctypes.c_double, _c_int,
+                                _c_int, _c_ptr]),
+    "pt_adamw8_moments": (_c_int, [_c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs, ctypes.POINTER(_c_i64),
+                                   _c_ptrs, _c_ptrs, _c_int, _c_ptr]),
     "pt_add_rmsnorm_fwd": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64,
                                     _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_int, _c_int,
                                     _c_float, _c_ptr]),
@@ -408,6 +434,102 @@ def cross_entropy_bwd(logits: int, vocab: int, outer: int, inner: int, logits_st
     _check("pt_cross_entropy_bwd", status, error_type)
 
 
+def logit_loss_workspace(vocab: int, outer: int, inner: int, dtype: int,
+                         error_type: type[Exception] | None = None) -> int:
+    """Bytes of device workspace that a logit loss's forward needs."""
+
+    out = _c_i64(0)
+    status = library().pt_logit_loss_workspace(vocab, outer, inner, dtype, ctypes.byref(out))
+    _check("pt_logit_loss_workspace", status, error_type)
+    return out.value
+
+
+# The wrappers below take rows(t) = (address, outer stride, inner stride) for each tensor that
+# has one entry or one row of logits per token.
+
+
+def token_logps_fwd(logits, vocab: int, outer: int, inner: int, targets, ignore_index: int,
+                    logps: int, stats: int, workspace: int, workspace_size: int, dtype: int,
+                    stream: int, error_type: type[Exception] | None = None) -> None:
+    """Log-probabilities of the targets (see pt_token_logps_fwd)."""
+
+    status = library().pt_token_logps_fwd(logits[0], vocab, outer, inner, logits[1], logits[2],
+                                          *targets, ignore_index, logps, stats, workspace,
+                                          workspace_size, dtype, stream)
+    _check("pt_token_logps_fwd", status, error_type)
+
+
+def token_logps_bwd(logits, vocab: int, outer: int, inner: int, targets, ignore_index: int,
+                    stats: int, coef, grad: int | None, dlogits, dtype: int, stream: int,
+                    error_type: type[Exception] | None = None) -> None:
+    """Logits gradient of any loss of the log-probabilities (see pt_token_logps_bwd)."""
+
+    status = library().pt_token_logps_bwd(logits[0], vocab, outer, inner, logits[1], logits[2],
+                                          *targets, ignore_index, stats, *coef, grad, *dlogits,
+                                          dtype, stream)
+    _check("pt_token_logps_bwd", status, error_type)
+
+
+def preference_loss_fwd(logits, vocab: int, outer: int, inner: int, targets, ignore_index: int,
+                        reference, beta: float, label_smoothing: float, loss: int, rewards: int,
+                        stats: int, coef: int, workspace: int, workspace_size: int, dtype: int,
+                        stream: int, error_type: type[Exception] | None = None) -> None:
+    """Preference loss of chosen / rejected pairs (see pt_preference_loss_fwd)."""
+
+    status = library().pt_preference_loss_fwd(logits[0], vocab, outer, inner, logits[1],
+                                              logits[2], *targets, ignore_index, *reference,
+                                              beta, label_smoothing, loss, rewards, stats, coef,
+                                              workspace, workspace_size, dtype, stream)
+    _check("pt_preference_loss_fwd", status, error_type)
+
+
+def policy_loss_fwd(logits, vocab: int, outer: int, inner: int, targets, ignore_index: int,
+                    old_logps, advantages, reference, clip_low: float, clip_high: float,
+                    kl_coef: float, by_sequence: bool, loss: int, logps: int, stats: int,
+                    coef: int, workspace: int, workspace_size: int, dtype: int, stream: int,
+                    error_type: type[Exception] | None = None) -> None:
+    """Clipped policy loss with an optional KL term (see pt_policy_loss_fwd)."""
+
+    status = library().pt_policy_loss_fwd(logits[0], vocab, outer, inner, logits[1], logits[2],
+                                          *targets, ignore_index, *old_logps, *advantages,
+                                          *reference, clip_low, clip_high, kl_coef,
+                                          int(bool(by_sequence)), loss, logps, stats, coef,
+                                          workspace, workspace_size, dtype, stream)
+    _check("pt_policy_loss_fwd", status, error_type)
+
+
+def _pointers(addresses) -> ctypes.Array:
+    return (_c_ptr * len(addresses))(*addresses)
+
+
+def adamw8_step(params, grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes,
+                exp_avg_sq_scales, numels, steps, lrs, weight_decays, beta1: float, beta2: float,
+                eps: float, maximize: bool, dtype: int, stream: int,
+                error_type: type[Exception] | None = None) -> None:
+    """One AdamW step with 8-bit states over lists of device addresses (see pt_adamw8_step)."""
+
+    n = len(params)
+    status = library().pt_adamw8_step(
+        _pointers(params), _pointers(grads), _pointers(exp_avg_codes), _pointers(exp_avg_scales),
+        _pointers(exp_avg_sq_codes), _pointers(exp_avg_sq_scales), (_c_i64 * n)(*numels),
+        (_c_i64 * n)(*steps), (ctypes.c_double * n)(*lrs), (ctypes.c_double * n)(*weight_decays),
+        n, float(beta1), float(beta2), float(eps), int(bool(maximize)), dtype, stream)
+    _check("pt_adamw8_step", status, error_type)
+
+
+def adamw8_moments(exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales, numels,
+                   exp_avgs, exp_avg_sqs, stream: int,
+                   error_type: type[Exception] | None = None) -> None:
+    """The fp32 moments of 8-bit states over lists of device addresses (pt_adamw8_moments)."""
+
+    n = len(numels)
+    status = library().pt_adamw8_moments(
+        _pointers(exp_avg_codes), _pointers(exp_avg_scales), _pointers(exp_avg_sq_codes),
+        _pointers(exp_avg_sq_scales), (_c_i64 * n)(*numels), _pointers(exp_avgs),
+        _pointers(exp_avg_sqs), n, stream)
+    _check("pt_adamw8_moments", status, error_type)
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, numels, steps, lrs, weight_decays,
                beta1: float, beta2: float, eps: float, maximize: bool, stream: int,
                error_type: type[Exception] | None = None) -> None:
@@ -435,6 +557,20 @@ def rope_qk(direction: str, q: int, q_strides, q_out: int, q_out_strides, q_size
                 _i64x4(k_strides), k_out, _i64x4(k_out_strides), _i64x4(k_sizes), cosine, sine,
                 table_row_stride, layout, dtype, table_dtype, stream)
     _check("pt_rope_qk_" + direction, status, error_type)
+
+
+def rope_positions(q: int, q_strides, q_out: int, q_out_strides, q_sizes, k: int, k_strides,
+                   k_out: int, k_out_strides, k_sizes, positions: int, position_strides,
+                   inv_freq: int, rotary_dim: int, scale: float, backward: bool, layout: int,
+                   dtype: int, stream: int, error_type: type[Exception] | None = None) -> None:
+    """Query and key rotated by explicit positions (see pt_rope_positions)."""
+
+    status = library().pt_rope_positions(
+        q, _i64x4(q_strides), q_out, _i64x4(q_out_strides), _i64x4(q_sizes), k,
+        _i64x4(k_strides), k_out, _i64x4(k_out_strides), _i64x4(k_sizes), positions,
+        position_strides[0], position_strides[1], inv_freq, rotary_dim, float(scale),
+        int(bool(backward)), layout, dtype, stream)
+    _check("pt_rope_positions", status, error_type)
 
 
 def selftest_wait_timeout(limit_cycles: int, stream: int) -> None:

@@ -29,3 +29,8 @@ class TritonCrossEntropyUnavailable(RuntimeError):
 
 class TritonAdamWUnavailable(RuntimeError):
     """The fused AdamW step cannot run this optimizer (reference triton_kernels/adamw.py:10)."""
+
+
+class TritonLogitLossUnavailable(RuntimeError):
+    """A loss over token log-probabilities cannot run these inputs (no reference counterpart:
+    its post-training losses are PyTorch code)."""

@@ -22,6 +22,7 @@ from torch.optim import Optimizer
 
 from picotron_b200 import _capi, ops
 from picotron_b200.errors import TritonAdamWUnavailable
+from picotron_b200.kernels.adamw8bit import AdamW8bit
 
 
 def _plan(optimizer: Optimizer):
@@ -103,7 +104,8 @@ class AdamWStepWithFallback:
 
     With ``use_triton`` the fused step runs; an optimizer it does not cover (see
     :func:`triton_adamw_step`) warns once with the reference's message and takes
-    ``optimizer.step()``, as the reference does. A missing library raises.
+    ``optimizer.step()``, as the reference does. An :class:`AdamW8bit`'s own step is the fused
+    one. A missing library raises.
     """
 
     def __init__(self, *, use_triton: bool = False) -> None:
@@ -111,7 +113,7 @@ class AdamWStepWithFallback:
         self._fallback_warned = False
 
     def step(self, optimizer: Optimizer) -> None:
-        if self.use_triton:
+        if self.use_triton and not isinstance(optimizer, AdamW8bit):
             try:
                 triton_adamw_step(optimizer)
                 return

@@ -9,7 +9,8 @@ Constructors, parameter names (and therefore checkpoint keys) and the
   (src/picotron/nn/feedforward.py:13-43), parameters
   ``{gate,up,down}_projection.weight``;
 * ``RotaryEmbedding(head_dim, theta=1e4, *, use_triton_rope=False)``
-  (src/picotron/nn/rope.py:54-107), no parameters.
+  (src/picotron/nn/rope.py:54-107), no parameters; beyond the reference,
+  ``forward`` takes explicit positions, and ``rotary_dim`` and ``scaling`` may be set.
 
 With the ``use_triton_*`` switch on and CUDA inputs, the sm_100a kernels run and any
 failure raises (there is no silent fallback on a GPU). With the switch on and non-CUDA
@@ -27,6 +28,7 @@ from torch import Tensor, nn
 from torch.nn import functional as F
 
 from picotron_b200 import ops
+from picotron_b200.kernels.rope import apply_rotary_positions, rotary_frequencies
 
 
 def _warn_once(module: nn.Module, what: str, error: Exception) -> None:
@@ -175,8 +177,27 @@ def apply_rotary_embedding(states: Tensor, cosine: Tensor, sine: Tensor) -> Tens
     return rotated.flatten(start_dim=-2)
 
 
+def _rotate_part(states: Tensor, cosine: Tensor, sine: Tensor) -> Tensor:
+    """Eager interleaved-pair rotation of the first 2 * cosine.size(-1) elements of each head, in
+    fp32 from tables that broadcast against (batch, heads, sequence)."""
+
+    rotated = 2 * cosine.size(-1)
+    wide = torch.promote_types(states.dtype, torch.float32)
+    cosine, sine = cosine.to(wide), sine.to(wide)
+    even, odd = states[..., 0:rotated:2].to(wide), states[..., 1:rotated:2].to(wide)
+    out = torch.stack((even * cosine - odd * sine, even * sine + odd * cosine), dim=-1)
+    return torch.cat((out.flatten(start_dim=-2).to(states.dtype), states[..., rotated:]), dim=-1)
+
+
 class RotaryEmbedding(nn.Module):
-    """Apply standard (interleaved-pair) RoPE to attention query and key tensors."""
+    """Apply (interleaved-pair) RoPE to attention query and key tensors.
+
+    The constructor is the reference's. Beyond it, ``forward`` takes explicit positions, and two
+    attributes may be set on the module: ``rotary_dim`` (only the first elements of each head are
+    rotated) and ``scaling`` (frequencies for long contexts: a dict of the keywords of
+    ``kernels.rotary_frequencies``, e.g. ``{"scaling": "yarn", "factor": 8.0,
+    "original_length": 4096}``).
+    """
 
     def __init__(
         self, head_dim: int, theta: float = 10_000.0, *, use_triton_rope: bool = False
@@ -189,10 +210,13 @@ class RotaryEmbedding(nn.Module):
         self.head_dim = head_dim
         self.theta = theta
         self.use_triton_rope = use_triton_rope
+        self.rotary_dim: int | None = None
+        self.scaling: dict | None = None
         self._triton_fallback_warned = False
         # Tables depend only on (S, D, theta, device, dtype); the reference rebuilds them
         # every call (nn/rope.py:79-85), this module builds each one once.
         self._tables: dict[tuple, tuple[Tensor, Tensor]] = {}
+        self._frequencies: dict[tuple, tuple[Tensor, float]] = {}
 
     def _cos_sin(self, sequence_length: int, device: torch.device, dtype: torch.dtype):
         key = (sequence_length, str(device), dtype)
@@ -204,8 +228,38 @@ class RotaryEmbedding(nn.Module):
             self._tables[key] = tables
         return tables
 
-    def forward(self, query: Tensor, key: Tensor) -> tuple[Tensor, Tensor]:
-        """Rotate query and key using their shared sequence positions."""
+    def _inverse_frequencies(self, device: torch.device) -> tuple[Tensor, float]:
+        """rotary_frequencies of the module's settings, built once per setting and device."""
+
+        rotary_dim = self.head_dim if self.rotary_dim is None else self.rotary_dim
+        if rotary_dim > self.head_dim:
+            raise ValueError("rotary_dim must be at most the attention head dimension.")
+        scaling = self.scaling or {}
+        key = (rotary_dim, self.theta, tuple(sorted(scaling.items())), str(device))
+        if key not in self._frequencies:
+            self._frequencies[key] = rotary_frequencies(rotary_dim, self.theta, device=device,
+                                                        **scaling)
+        return self._frequencies[key]
+
+    def _by_positions(self, query: Tensor, key: Tensor,
+                      positions: Tensor | None) -> tuple[Tensor, Tensor]:
+        if positions is None:
+            positions = torch.arange(query.size(-2), device=query.device)
+        frequencies, scale = self._inverse_frequencies(query.device)
+        if self.use_triton_rope:
+            if query.is_cuda and key.is_cuda:
+                return apply_rotary_positions(query, key, positions, frequencies, scale=scale)
+            _warn_once(self, "RoPE", RuntimeError("sm_100a RoPE requires CUDA tensors."))
+        angles = positions.unsqueeze(-1).double() * frequencies
+        if positions.dim() == 2:
+            angles = angles.unsqueeze(1)  # one row of angles for all heads
+        cosine, sine = angles.cos() * scale, angles.sin() * scale
+        return (_rotate_part(query, cosine, sine), _rotate_part(key, cosine, sine))
+
+    def forward(self, query: Tensor, key: Tensor,
+                positions: Tensor | None = None) -> tuple[Tensor, Tensor]:
+        """Rotate query and key using their shared sequence positions: 0 .. S-1, or the int64
+        ``positions`` ([S] or [B, S]), in any order and however far."""
 
         if (
             query.size(0) != key.size(0)
@@ -213,6 +267,8 @@ class RotaryEmbedding(nn.Module):
             or query.size(-1) != key.size(-1)
         ):
             raise ValueError("RoPE query and key must share batch, sequence, and head dimensions.")
+        if positions is not None or self.scaling or self.rotary_dim not in (None, self.head_dim):
+            return self._by_positions(query, key, positions)
         cosine, sine = self._cos_sin(query.size(-2), query.device, query.dtype)
         if self.use_triton_rope:
             if query.is_cuda and key.is_cuda:

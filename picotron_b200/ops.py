@@ -16,10 +16,15 @@ backward op:
 * ``cross_entropy(logits, targets, ignore_index) -> (loss, row_lse, mean_out)``
   (reference train_loop.py:95-97,141-145: F.cross_entropy, mean over non-ignored rows)
 * ``cross_entropy_backward(grad, logits, targets, row_lse, mean_out, ignore_index) -> dlogits``
+* ``token_logps(logits, targets, ignore_index) -> (logps, stats)``, ``preference_loss(...)`` and
+  ``policy_loss(...)``: post-training losses over the targets' log-probabilities, and
+  ``logit_loss_backward``, the logits gradient of all three
 * ``rope(x, cosine, sine, layout) -> out``           (reference nn/rope.py:35-51)
 * ``rope_backward(dy, cosine, sine, layout) -> dx``
 * ``rope_qk(q, k, cosine, sine, layout) -> (q_out, k_out)``  (query and key in one launch,
   reference nn/rope.py:70-107) and ``rope_qk_backward``
+* ``rope_positions(q, k, positions, inv_freq, layout, scale) -> (q_out, k_out)`` (query and key
+  by explicit positions, part of the head) and ``rope_positions_backward``
 
 All ops run only on CUDA tensors of a compute-capability-10.0 device and launch on the
 current stream of the tensors' device. Any failure raises the reference's exception
@@ -34,6 +39,7 @@ from torch import Tensor
 from picotron_b200 import _capi
 from picotron_b200.errors import (
     TritonCrossEntropyUnavailable,
+    TritonLogitLossUnavailable,
     TritonRMSNormUnavailable,
     TritonRoPEUnavailable,
     TritonSwiGLUUnavailable,
@@ -643,6 +649,270 @@ def _ce_backward(ctx, grad, _grad_lse, _grad_mean):
 cross_entropy.register_autograd(_ce_backward, setup_context=_ce_setup)
 
 
+# ------------------------------------------------------ losses over log-probabilities --
+
+
+def _ll_geometry(logits: Tensor, targets: Tensor) -> tuple[int, int]:
+    """(sequences, positions) of logits [B, S, V] with targets [B, S]; logits [N, V] with targets
+    [N] are one sequence."""
+
+    if logits.dim() == 2 and targets.shape == logits.shape[:1]:
+        return 1, logits.size(0)
+    if logits.dim() == 3 and targets.shape == logits.shape[:2]:
+        return logits.size(0), logits.size(1)
+    raise TritonLogitLossUnavailable(
+        "expected logits [N, V] with targets [N], or logits [B, S, V] with targets [B, S]; got "
+        f"{tuple(logits.shape)} and {tuple(targets.shape)}")
+
+
+def _ll_rows(t: Tensor) -> tuple[int, int, int]:
+    """Address and the two row strides of a tensor with one entry (or row) per token."""
+
+    if t.dim() == 1:
+        return t.data_ptr(), 0, t.stride(0)
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _ll_logits(logits: Tensor) -> Tensor:
+    """Logits with a contiguous class dimension and rows that do not overlap, copied if needed."""
+
+    if logits.stride(-1) != 1 and logits.size(-1) > 1:
+        return logits.contiguous()
+    reach = logits.size(-1)
+    dims = sorted((logits.stride(d), logits.size(d)) for d in range(logits.dim() - 1)
+                  if logits.size(d) > 1)
+    for stride, size in dims:
+        if stride < reach:
+            return logits.contiguous()
+        reach = stride * (size - 1) + reach
+    return logits
+
+
+def _ll_inputs(logits: Tensor, targets: Tensor, per_token=()) -> tuple[Tensor, int, int]:
+    check_device(logits.device, TritonLogitLossUnavailable)
+    _dtype_code(logits, TritonLogitLossUnavailable)
+    outer, inner = _ll_geometry(logits, targets)
+    if targets.dtype != torch.long:
+        raise TritonLogitLossUnavailable("targets must be int64 class indices.")
+    if logits.size(-1) < 1:
+        raise TritonLogitLossUnavailable("logits need at least one class.")
+    for t in (targets, *per_token):
+        if t.device != logits.device:
+            raise TritonLogitLossUnavailable("all tensors must be on the logits' device.")
+    for t in per_token:
+        if t.dtype != torch.float32 or t.shape != targets.shape:
+            raise TritonLogitLossUnavailable(
+                "per-token inputs must be float32 and have the targets' shape.")
+    return _ll_logits(logits), outer, inner
+
+
+def _ll_logits_rows(logits: Tensor) -> tuple[int, int, int]:
+    if logits.dim() == 2:
+        return logits.data_ptr(), 0, logits.stride(0)
+    return logits.data_ptr(), logits.stride(0), logits.stride(1)
+
+
+def _ll_workspace(logits: Tensor, outer: int, inner: int) -> Tensor:
+    size = _capi.logit_loss_workspace(logits.size(-1), outer, inner, DTYPE_CODES[logits.dtype],
+                                      TritonLogitLossUnavailable)
+    return torch.empty(max(size, 16), dtype=torch.uint8, device=logits.device)
+
+
+def _ll_dense_gradient(logits: Tensor) -> bool:
+    """Whether a contiguous gradient's rows sit at the same offsets modulo 16 bytes."""
+
+    size = logits.element_size()
+    return logits.is_contiguous() or all(
+        n * size % 16 == 0
+        for n in (logits.size(-1), *(logits.stride(d) for d in range(logits.dim() - 1)
+                                     if logits.size(d) > 1)))
+
+
+def _ll_gradient(logits: Tensor) -> Tensor:
+    """An empty gradient whose rows have the addresses of the logits' rows modulo 16 bytes, so that
+    both are read and written in the same whole vectors: contiguous, or with the strides of a
+    strided view of odd-sized rows."""
+
+    shift = logits.data_ptr() % 16 // logits.element_size()
+    if _ll_dense_gradient(logits):
+        strides, span = torch.empty(logits.shape, device="meta").stride(), logits.numel()
+    else:
+        strides = logits.stride()
+        span = 1 + sum((n - 1) * st for n, st in zip(logits.shape, strides))
+    buffer = torch.empty(span + shift, dtype=logits.dtype, device=logits.device)
+    return buffer.as_strided(logits.shape, strides, shift)
+
+
+@torch.library.custom_op("picotron_b200::token_logps", mutates_args=())
+def token_logps(logits: Tensor, targets: Tensor, ignore_index: int) -> tuple[Tensor, Tensor]:
+    x, outer, inner = _ll_inputs(logits, targets)
+    logps = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    stats = torch.empty((*targets.shape, 2), dtype=torch.float32, device=x.device)
+    if targets.numel() == 0:
+        return logps, stats
+    with _OnDevice(x.device):
+        work = _ll_workspace(x, outer, inner)
+        _capi.token_logps_fwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
+                              int(ignore_index), logps.data_ptr(), stats.data_ptr(),
+                              work.data_ptr(), work.numel(), DTYPE_CODES[x.dtype],
+                              _stream(x.device), TritonLogitLossUnavailable)
+    return logps, stats
+
+
+@token_logps.register_fake
+def _token_logps_fake(logits, targets, ignore_index):
+    return (torch.empty(targets.shape, dtype=torch.float32, device=logits.device),
+            torch.empty((*targets.shape, 2), dtype=torch.float32, device=logits.device))
+
+
+@torch.library.custom_op("picotron_b200::logit_loss_backward", mutates_args=())
+def logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: Tensor,
+                        grad: Tensor | None, ignore_index: int) -> Tensor:
+    """dlogits = coef * grad * (onehot(targets) - softmax(logits)); coef has the targets' shape
+    (and any strides), grad is one value."""
+
+    x, outer, inner = _ll_inputs(logits, targets, (coef,))
+    if stats.shape != (*targets.shape, 2) or not stats.is_contiguous():
+        raise TritonLogitLossUnavailable("stats must be the forward's.")
+    dlogits = _ll_gradient(x)
+    if dlogits.numel() == 0:
+        return dlogits
+    if grad is not None:
+        grad = grad.to(torch.float32)
+    with _OnDevice(x.device):
+        _capi.token_logps_bwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
+                              int(ignore_index), stats.data_ptr(), _ll_rows(coef),
+                              grad.data_ptr() if grad is not None else None,
+                              _ll_logits_rows(dlogits), DTYPE_CODES[x.dtype], _stream(x.device),
+                              TritonLogitLossUnavailable)
+    return dlogits
+
+
+@logit_loss_backward.register_fake
+def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
+    x = _ll_logits(logits)
+    if _ll_dense_gradient(x):
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+
+
+def _token_logps_setup(ctx, inputs, output) -> None:
+    logits, targets, ctx.ignore_index = inputs
+    ctx.save_for_backward(logits, targets, output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _token_logps_bwd(ctx, grad, _grad_stats):
+    if grad is None:
+        return None, None, None
+    logits, targets, stats = ctx.saved_tensors
+    return torch.ops.picotron_b200.logit_loss_backward(logits, targets, stats, grad, None,
+                                                       ctx.ignore_index), None, None
+
+
+token_logps.register_autograd(_token_logps_bwd, setup_context=_token_logps_setup)
+
+
+@torch.library.custom_op("picotron_b200::preference_loss", mutates_args=())
+def preference_loss(logits: Tensor, targets: Tensor, reference: Tensor, beta: float,
+                    label_smoothing: float,
+                    ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(loss, rewards, stats, coef) of pt_preference_loss_fwd."""
+
+    x, outer, inner = _ll_inputs(logits, targets, (reference,))
+    if logits.dim() != 3 or outer % 2 != 0:
+        raise TritonLogitLossUnavailable(
+            "preference loss expects logits [2P, S, V]: P chosen sequences, then their P rejected")
+    loss = torch.empty((), dtype=torch.float32, device=x.device)
+    rewards = torch.empty(outer, dtype=torch.float32, device=x.device)
+    stats = torch.empty((*targets.shape, 2), dtype=torch.float32, device=x.device)
+    coef = torch.empty(outer, dtype=torch.float32, device=x.device)
+    with _OnDevice(x.device):
+        work = _ll_workspace(x, outer, inner)
+        _capi.preference_loss_fwd(_ll_logits_rows(x), x.size(-1), outer, inner,
+                                  _ll_rows(targets), int(ignore_index), _ll_rows(reference),
+                                  float(beta), float(label_smoothing), loss.data_ptr(),
+                                  rewards.data_ptr(), stats.data_ptr(), coef.data_ptr(),
+                                  work.data_ptr(), work.numel(), DTYPE_CODES[x.dtype],
+                                  _stream(x.device), TritonLogitLossUnavailable)
+    return loss, rewards, stats, coef
+
+
+@preference_loss.register_fake
+def _preference_loss_fake(logits, targets, reference, beta, label_smoothing, ignore_index):
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
+    return new(), new(logits.size(0)), new(*targets.shape, 2), new(logits.size(0))
+
+
+def _preference_setup(ctx, inputs, output) -> None:
+    logits, targets, _, _, _, ctx.ignore_index = inputs
+    ctx.save_for_backward(logits, targets, output[2], output[3])
+    ctx.set_materialize_grads(False)
+
+
+def _preference_bwd(ctx, grad, *_):
+    if grad is None:
+        return (None,) * 6
+    logits, targets, stats, coef = ctx.saved_tensors
+    dlogits = torch.ops.picotron_b200.logit_loss_backward(
+        logits, targets, stats, coef[:, None].expand(targets.shape), grad, ctx.ignore_index)
+    return dlogits, None, None, None, None, None
+
+
+preference_loss.register_autograd(_preference_bwd, setup_context=_preference_setup)
+
+
+@torch.library.custom_op("picotron_b200::policy_loss", mutates_args=())
+def policy_loss(logits: Tensor, targets: Tensor, old_logps: Tensor, advantages: Tensor,
+                reference: Tensor | None, clip_low: float, clip_high: float, kl_coef: float,
+                by_sequence: bool,
+                ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(loss, logps, stats, coef) of pt_policy_loss_fwd."""
+
+    per_token = (old_logps, advantages) if reference is None else (old_logps, advantages, reference)
+    x, outer, inner = _ll_inputs(logits, targets, per_token)
+    loss = torch.empty((), dtype=torch.float32, device=x.device)
+    logps = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    stats = torch.empty((*targets.shape, 2), dtype=torch.float32, device=x.device)
+    coef = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    with _OnDevice(x.device):
+        work = _ll_workspace(x, outer, inner)
+        _capi.policy_loss_fwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
+                              int(ignore_index), _ll_rows(old_logps), _ll_rows(advantages),
+                              _ll_rows(reference) if reference is not None else (None, 0, 0),
+                              float(clip_low), float(clip_high), float(kl_coef),
+                              by_sequence, loss.data_ptr(), logps.data_ptr(), stats.data_ptr(),
+                              coef.data_ptr(), work.data_ptr(), work.numel(),
+                              DTYPE_CODES[x.dtype], _stream(x.device),
+                              TritonLogitLossUnavailable)
+    return loss, logps, stats, coef
+
+
+@policy_loss.register_fake
+def _policy_loss_fake(logits, targets, old_logps, advantages, reference, clip_low, clip_high,
+                      kl_coef, by_sequence, ignore_index):
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
+    return new(), new(*targets.shape), new(*targets.shape, 2), new(*targets.shape)
+
+
+def _policy_setup(ctx, inputs, output) -> None:
+    ctx.ignore_index = inputs[-1]
+    ctx.save_for_backward(inputs[0], inputs[1], output[2], output[3])
+    ctx.set_materialize_grads(False)
+
+
+def _policy_bwd(ctx, grad, *_):
+    if grad is None:
+        return (None,) * 10
+    logits, targets, stats, coef = ctx.saved_tensors
+    dlogits = torch.ops.picotron_b200.logit_loss_backward(logits, targets, stats, coef, grad,
+                                                          ctx.ignore_index)
+    return (dlogits, *(None,) * 9)
+
+
+policy_loss.register_autograd(_policy_bwd, setup_context=_policy_setup)
+
+
 # ------------------------------------------------------------------------------ RoPE --
 
 
@@ -803,3 +1073,91 @@ def _rope_qk_bwd(ctx, dq: Tensor | None, dk: Tensor | None):
 
 
 rope_qk.register_autograd(_rope_qk_bwd, setup_context=_rope_qk_setup)
+
+
+def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tensor,
+                           inv_freq: Tensor, layout: int, scale: float) -> tuple[Tensor, Tensor]:
+    check_device(q.device, TritonRoPEUnavailable)
+    for t in (k, positions, inv_freq):
+        if t.device != q.device:
+            raise TritonRoPEUnavailable("RoPE query, key, positions and frequencies must share a "
+                                        "device.")
+    if layout not in (_capi.PT_ROPE_INTERLEAVED, _capi.PT_ROPE_ROTATE_HALF):
+        raise TritonRoPEUnavailable(f"unknown RoPE layout {layout}")
+    code = _dtype_code(q, TritonRoPEUnavailable)
+    if q.dim() != 4 or k.dim() != 4 or k.dtype != q.dtype or (
+            q.size(0), q.size(2), q.size(3)) != (k.size(0), k.size(2), k.size(3)):
+        raise TritonRoPEUnavailable("RoPE requires query and key [B, H, S, D] of one dtype that "
+                                    "share B, S and D.")
+    if positions.dtype != torch.long or positions.shape not in ((q.size(2),),
+                                                                (q.size(0), q.size(2))):
+        raise TritonRoPEUnavailable("RoPE positions must be int64 [S] or [B, S].")
+    if (inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.numel() < 1
+            or 2 * inv_freq.numel() > q.size(3)):
+        raise TritonRoPEUnavailable("RoPE frequencies must be float64 [R/2] with R at most the "
+                                    "head dimension.")
+    q, q_out = _rope_state(q)
+    k, k_out = _rope_state(k)
+    if q.size(0) * q.size(2) == 0 or q.numel() + k.numel() == 0:
+        return q_out, k_out
+    strides = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    inv_freq = inv_freq.contiguous()
+    with _OnDevice(q.device):
+        _capi.rope_positions(q.data_ptr(), q.stride(), q_out.data_ptr(), q_out.stride(), q.shape,
+                             k.data_ptr(), k.stride(), k_out.data_ptr(), k_out.stride(), k.shape,
+                             positions.data_ptr(), strides, inv_freq.data_ptr(),
+                             2 * inv_freq.numel(), scale, backward, layout, code,
+                             _stream(q.device), TritonRoPEUnavailable)
+    return q_out, k_out
+
+
+def _rope_state(x: Tensor) -> tuple[Tensor, Tensor]:
+    """States with a contiguous head dimension, and the output: the same memory layout when that
+    is dense, else contiguous."""
+
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    out = torch.empty_like(x)
+    return x, out if out.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+@torch.library.custom_op("picotron_b200::rope_positions", mutates_args=())
+def rope_positions(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, layout: int,
+                   scale: float) -> tuple[Tensor, Tensor]:
+    return _rope_positions_launch(False, q, k, positions, inv_freq, layout, scale)
+
+
+@torch.library.custom_op("picotron_b200::rope_positions_backward", mutates_args=())
+def rope_positions_backward(dq: Tensor, dk: Tensor, positions: Tensor, inv_freq: Tensor,
+                            layout: int, scale: float) -> tuple[Tensor, Tensor]:
+    return _rope_positions_launch(True, dq, dk, positions, inv_freq, layout, scale)
+
+
+def _rope_positions_fake(q, k, positions, inv_freq, layout, scale):
+    return _rope_state(q)[1], _rope_state(k)[1]
+
+
+rope_positions.register_fake(_rope_positions_fake)
+rope_positions_backward.register_fake(_rope_positions_fake)
+
+
+def _rope_positions_setup(ctx, inputs, output) -> None:
+    q, k, positions, inv_freq, ctx.layout, ctx.scale = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.q_meta = (q.shape, q.dtype, q.device)
+    ctx.k_meta = (k.shape, k.dtype, k.device)
+    ctx.set_materialize_grads(False)
+
+
+def _rope_positions_bwd(ctx, dq: Tensor | None, dk: Tensor | None):
+    positions, inv_freq = ctx.saved_tensors
+    if dq is None:
+        dq = torch.zeros(ctx.q_meta[0], dtype=ctx.q_meta[1], device=ctx.q_meta[2])
+    if dk is None:
+        dk = torch.zeros(ctx.k_meta[0], dtype=ctx.k_meta[1], device=ctx.k_meta[2])
+    gq, gk = torch.ops.picotron_b200.rope_positions_backward(dq, dk, positions, inv_freq,
+                                                             ctx.layout, ctx.scale)
+    return gq, gk, None, None, None, None
+
+
+rope_positions.register_autograd(_rope_positions_bwd, setup_context=_rope_positions_setup)
