@@ -457,6 +457,36 @@ PT_API int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, 
                               float* stats, float* coef, void* workspace, int64_t workspace_size,
                               int dtype, void* stream);
 
+/* pt_policy_loss_fwd and, in the same pass over the logits, dlogits = grad * d loss / d logits,
+ * for a caller that knows (or expects) the factor `grad` that the loss's gradient will have:
+ * rows stay on chip between their statistics and their gradient, so the logits are read once
+ * instead of twice. stats and coef are written as well (coef without the factor). dlogits as in
+ * pt_token_logps_bwd. Rows of more than 1.5 MiB, or more than 2^28 rows, are refused:
+ * pt_policy_loss_grad_supported says so beforehand. A bounded wait that runs out sets the device
+ * error word (code 1). */
+PT_API int pt_policy_loss_grad_supported(int64_t vocab, int64_t outer, int64_t inner, int dtype,
+                                         int* supported);
+PT_API int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                               int64_t logits_outer_stride, int64_t logits_inner_stride,
+                               const int64_t* targets, int64_t targets_outer_stride,
+                               int64_t targets_inner_stride, int64_t ignore_index,
+                               const float* old_logps, int64_t old_outer_stride,
+                               int64_t old_inner_stride, const float* advantages,
+                               int64_t advantages_outer_stride, int64_t advantages_inner_stride,
+                               const float* reference, int64_t reference_outer_stride,
+                               int64_t reference_inner_stride, double clip_low, double clip_high,
+                               double kl_coef, int by_sequence, double grad, float* loss,
+                               float* logps, float* stats, float* coef, void* dlogits,
+                               int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
+                               void* workspace, int64_t workspace_size, int dtype, void* stream);
+
+/* Multiplies a gradient that was formed for the factor `expected` (finite, not 0) by *grad /
+ * expected, in place; *grad is one fp32 value in device memory, and where it equals expected
+ * nothing is read or written. */
+PT_API int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t inner,
+                                  int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
+                                  const float* grad, double expected, int dtype, void* stream);
+
 /* ------------------------------------------------------------------ AdamW -------- */
 
 /* One fused AdamW step over num_tensors fp32 parameters (device pointers in host arrays):

@@ -119,6 +119,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pt_policy_loss_fwd": (_c_int, [*_LOGITS, *_ROWS, *_ROWS, *_ROWS, ctypes.c_double,
                                     ctypes.c_double, ctypes.c_double, _c_int, _c_ptr, _c_ptr,
                                     _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
+    "pt_policy_loss_grad_supported": (_c_int, [_c_i64, _c_i64, _c_i64, _c_int,
+                                               ctypes.POINTER(_c_int)]),
+    "pt_policy_loss_grad": (_c_int, [*_LOGITS, *_ROWS, *_ROWS, *_ROWS, ctypes.c_double,
+                                     ctypes.c_double, ctypes.c_double, _c_int, ctypes.c_double,
+                                     _c_ptr, _c_ptr, _c_ptr, _c_ptr, *_ROWS, _c_ptr, _c_i64,
+                                     _c_int, _c_ptr]),
+    "pt_rescale_logits_grad": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr,
+                                        ctypes.c_double, _c_int, _c_ptr]),
     "pt_adamw8_step": (_c_int, [_c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs, _c_ptrs,
                                 ctypes.POINTER(_c_i64), ctypes.POINTER(_c_i64),
                                 ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),
@@ -496,6 +504,40 @@ def policy_loss_fwd(logits, vocab: int, outer: int, inner: int, targets, ignore_
                                           int(bool(by_sequence)), loss, logps, stats, coef,
                                           workspace, workspace_size, dtype, stream)
     _check("pt_policy_loss_fwd", status, error_type)
+
+
+def policy_loss_grad_supported(vocab: int, outer: int, inner: int, dtype: int,
+                               error_type: type[Exception] | None = None) -> bool:
+    out = _c_int(0)
+    status = library().pt_policy_loss_grad_supported(vocab, outer, inner, dtype,
+                                                     ctypes.byref(out))
+    _check("pt_policy_loss_grad_supported", status, error_type)
+    return bool(out.value)
+
+
+def policy_loss_grad(logits, vocab: int, outer: int, inner: int, targets, ignore_index: int,
+                     old_logps, advantages, reference, clip_low: float, clip_high: float,
+                     kl_coef: float, by_sequence: bool, grad: float, loss: int, logps: int,
+                     stats: int, coef: int, dlogits, workspace: int, workspace_size: int,
+                     dtype: int, stream: int, error_type: type[Exception] | None = None) -> None:
+    """The policy loss and its logits gradient in one pass (see pt_policy_loss_grad)."""
+
+    status = library().pt_policy_loss_grad(logits[0], vocab, outer, inner, logits[1], logits[2],
+                                           *targets, ignore_index, *old_logps, *advantages,
+                                           *reference, clip_low, clip_high, kl_coef,
+                                           int(bool(by_sequence)), grad, loss, logps, stats, coef,
+                                           *dlogits, workspace, workspace_size, dtype, stream)
+    _check("pt_policy_loss_grad", status, error_type)
+
+
+def rescale_logits_grad(dlogits, vocab: int, outer: int, inner: int, grad: int, expected: float,
+                        dtype: int, stream: int,
+                        error_type: type[Exception] | None = None) -> None:
+    """A gradient formed for another factor than it gets (see pt_rescale_logits_grad)."""
+
+    status = library().pt_rescale_logits_grad(dlogits[0], vocab, outer, inner, dlogits[1],
+                                              dlogits[2], grad, expected, dtype, stream)
+    _check("pt_rescale_logits_grad", status, error_type)
 
 
 def _pointers(addresses) -> ctypes.Array:

@@ -2,13 +2,15 @@
 // (forward and backward), the preference loss of chosen / rejected pairs and the clipped policy
 // loss with a KL term, each with the gradient of its logits.
 //
-// For a row x with target t:
-//   m = max(x),  s = sum 2^((x - m) log2 e),  log softmax(x)_t = (x_t - m) - ln s.
+// For a row x with target t, relative to a reference m near max(x):
+//   s = sum 2^((x - m) log2 e),  log softmax(x)_t = (x_t - m) - ln s.
 // x is taken relative to m before it is scaled, so a row of one type's lowest values (a mask
-// that leaves nothing) neither overflows nor loses its s; s is held in 32 bits per thread and
-// merged in 32 bits, ln s and the differences are taken in 64 bits and the log-probability is
-// rounded once. Every loss here depends on the logits through these log-probabilities alone,
-// so its gradient is
+// that leaves nothing) neither overflows nor loses its s. Losses sum these over thousands of
+// positions, where a bias matters more than a rounding: log2 e is applied in two parts, the mean
+// error of the exponential unit is taken out of each term, and sums are rescaled only when the
+// reference has fallen e^8 behind and once more when threads are merged. The differences are
+// taken in 64 bits and the log-probability is rounded once. Every loss here depends on the
+// logits through these log-probabilities alone, so its gradient is
 //   dx = c (onehot(t) - softmax(x)),  softmax(x) = 2^((x - m) log2 e) / s,
 // with one coefficient c per row: the forward keeps (m, 1/s) and c, the backward reads the
 // logits once more and writes dx. All passes over the logits are bound by HBM bandwidth.
@@ -27,13 +29,25 @@ __device__ int g_logit_loss_error = 0;
 
 namespace {
 
-// Rows per CTA and vectors in flight as for the cross-entropy kernels, which read the same
-// rows: 128 threads, 8 vectors in flight where rows are only read, 4 where dx is written too.
-constexpr int kThreads = 128;
+// Vectors in flight per thread as for the cross-entropy kernels, which read the same rows: 8
+// where rows are only read, 4 where dx is written too.
+#ifndef PT_LL_THREADS
+#define PT_LL_THREADS 128
+#endif
+#ifndef PT_LL_TRIPS
+#define PT_LL_TRIPS 4
+#endif
+constexpr int kThreads = PT_LL_THREADS;
+constexpr int kGradTrips = PT_LL_TRIPS;  // unrolled trips per CTA of the gradient
 constexpr int kUnrollStats = 8;
 constexpr int kUnrollGrad = 4;
 constexpr int kSumThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f;  // log2(e): exp(a) = 2^(a log2(e))
+constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);  // what it lacks
+// How far ex2.approx is below the true value on average (measured over 4 M points of [-20, 0] on
+// B200; its largest error is 1.4e-7). e + e kExpLow, rounded, adds about that much on average.
+constexpr float kExpLow = 5.05e-8f;
+constexpr float kRaise = 8.0f;  // how far a value may pass the reference: e^8 V stays in range
 constexpr int kErrBadTarget = 2;
 
 // Row r of the [outer, inner] row grid sits at outer index r / inner, inner index r % inner.
@@ -53,43 +67,48 @@ struct Targets {
   __device__ __forceinline__ int64_t at(int64_t r) const { return p[g.offset(r)]; }
 };
 
-// A set of values x as (max, sum of e^(x - max)); m = -inf and s = 0 for the empty set.
+// A set of values x as (reference m, sum of e^(x - m)); m = -inf and s = 0 for the empty set.
 struct Stat {
   float m, s;
 };
 
-// 2^x on the special-function unit (PTX ex2.approx.ftz, relative error below 2^-22).
+// 2^x on the special-function unit (PTX ex2.approx.ftz).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float fast_exp(float a) { return fast_exp2(a * kLog2e); }
-
-__device__ __forceinline__ Stat merge(Stat a, Stat b) {
-  const float m = fmaxf(a.m, b.m);
-  const float fa = a.m == -INFINITY ? 0.0f : fast_exp(a.m - m);
-  const float fb = b.m == -INFINITY ? 0.0f : fast_exp(b.m - m);
-  // A NaN sum survives even where its factor is 0 (NaN * 0).
-  return {m, fmaf(a.s, fa, b.s * fb)};
+__device__ __forceinline__ float2 log2_scaled(float2 d) {  // d log2(e)
+  return __ffma2_rn(d, splat2(kLog2e), __fmul2_rn(d, splat2(kLog2eLow)));
+}
+__device__ __forceinline__ float fast_exp(float d) {
+  const float y = fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+  return fmaf(y, kExpLow, y);
 }
 
-__device__ __forceinline__ Stat warp_merge(Stat v) {
+// The sum of v relative to the reference m >= v.m. A NaN sum stays NaN (NaN * 0).
+__device__ __forceinline__ float sum_at(Stat v, float m) {
+  return v.m == m ? v.s : v.s * (v.m == -INFINITY ? 0.0f : fast_exp(v.m - m));
+}
+
+__device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1)
-    v = merge(v, Stat{__shfl_xor_sync(0xffffffffu, v.m, off),
-                      __shfl_xor_sync(0xffffffffu, v.s, off)});
+  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
 
-// Merged over the CTA; valid in warp 0. `red` holds one Stat per warp.
+// Merged over the CTA; valid in all threads of warp 0. `red` holds one Stat per warp.
 __device__ __forceinline__ Stat block_merge(Stat v, Stat* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  v = warp_merge(v);
-  if (lane == 0) red[warp] = v;
+  const float wm = warp_max(v.m);
+  if (lane == 0) red[warp].m = wm;
   __syncthreads();
-  if (warp == 0) v = warp_merge(lane < nw ? red[lane] : Stat{-INFINITY, 0.0f});
-  return v;
+  float m = red[0].m;
+  for (int w = 1; w < nw; ++w) m = fmaxf(m, red[w].m);
+  const float ws = warp_sum(sum_at(v, m));
+  if (lane == 0) red[warp].s = ws;
+  __syncthreads();
+  return {m, warp == 0 ? warp_sum(lane < nw ? red[lane].s : 0.0f) : 0.0f};
 }
 
 // Per-thread running statistics: two partial sums (paired fp32 lanes) relative to m.
@@ -97,7 +116,7 @@ struct Running {
   float m = -INFINITY;
   float2 s = make_float2(0.0f, 0.0f);
   __device__ __forceinline__ void raise(float xmax) {
-    if (xmax > m) {
+    if (xmax > m + kRaise || m == -INFINITY) {
       s = __fmul2_rn(s, splat2(m == -INFINITY ? 0.0f : fast_exp(m - xmax)));
       m = xmax;
     }
@@ -110,11 +129,12 @@ struct Running {
 #pragma unroll
     for (int e = 1; e < N; ++e) vmax = fmaxf(vmax, x[e]);
     raise(vmax);
-    const float2 L = splat2(kLog2e), nm = splat2(-base());
+    const float2 nm = splat2(-base());
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
-      const float2 t = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm), L);
-      s = __fadd2_rn(s, make_float2(fast_exp2(t.x), fast_exp2(t.y)));
+      const float2 t = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm));
+      const float2 y = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+      s = __fadd2_rn(s, __ffma2_rn(y, splat2(kExpLow), y));
     }
   }
   __device__ __forceinline__ void add1(float x) {
@@ -125,9 +145,16 @@ struct Running {
 };
 
 // log softmax at the value xt. The differences are taken first: m may be as large as the type
-// allows, where m + ln s would absorb ln s.
+// allows, where m + ln s would absorb ln s. s = 2^k f with f in [2^-1/2, 2^1/2): k ln 2 is exact in
+// 64 bits and the fp32 logarithm of f is within 2^-25 (a 64-bit one took longer than a short
+// row's pass).
 __device__ __forceinline__ double log_softmax(Stat v, float xt) {
-  return ((double)xt - (double)v.m) - log((double)v.s);
+  const int bits = __float_as_int(v.s) - 0x3f3504f3;  // of 2^-1/2
+  const int k = bits >> 23;
+  const float f = __int_as_float((bits & 0x007fffff) + 0x3f3504f3);
+  // s - s is 0, or NaN where s is not finite and has no such k and f.
+  return ((double)xt - (double)v.m) -
+         ((double)k * 0.6931471805599453 + (double)(logf(f) + (v.s - v.s)));
 }
 
 // Elements before the first 16-byte boundary of a row (0 when it is aligned).
@@ -247,15 +274,20 @@ finish_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows
     float xt = 0.0f;
     if (kind == kRowUsed) {
       xt = to_float(logits[lg.offset(r) + t]);
-      for (int k = lane; k < splits; k += 32) v = merge(v, part[r * splits + k]);
-      v = warp_merge(v);
+      for (int k = lane; k < splits; k += 32) v.m = fmaxf(v.m, part[r * splits + k].m);
+      v.m = warp_max(v.m);
+      for (int k = lane; k < splits; k += 32) v.s += sum_at(part[r * splits + k], v.m);
+      v.s = warp_sum(v.s);
     }
     if (lane == 0) out.store(r, kind, v, xt);
   }
 }
 
-// dx = c (onehot - softmax), one CTA per (row, split); c = coef[row] * grad. Rows are visited
-// from the last to the first: the forward read the last ones last, so they are still in L2.
+// dx = c (onehot - softmax), one CTA per (row, split); c = coef[row] * grad. A split is kGradTrips
+// unrolled trips: rows without a target cost a fraction of the others, so CTAs have to be short
+// and handed out as they finish (one row per CTA in a fixed assignment took 1.45 times as long
+// at 8192 x 128256 bf16 with a third of the rows ignored). Rows are visited from the last to
+// the first: the forward read the last ones last, so they are still in L2.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, int64_t vocab,
@@ -294,13 +326,13 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
       const float e = fast_exp(to_float(row[col]) + nm);
       drow[col] = from_float<T>(col == t ? fmaf(a, e, c) : a * e);
     };
-    const float2 L = splat2(kLog2e), nm2 = splat2(nm), a2 = splat2(a);
+    const float2 nm2 = splat2(nm), a2 = splat2(a);
     auto vec = [&](const uint4& raw, int64_t v) {
       float x[V];
       unpack<T>(raw, x);
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2), L);
+        const float2 y = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2));
         x[e] = fast_exp2(y.x);
         x[e + 1] = fast_exp2(y.y);
       }
@@ -435,37 +467,51 @@ struct PolicyTerms {
   float* coef;      // [rows] d loss / d logp
 };
 
-// max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
-// derivative to lp; -A r where the unclipped term is the larger one.
-__device__ __forceinline__ void policy_term(const PolicyTerms& p, int64_t r, double lp, double w,
-                                            double& term, double& coef) {
-  const double a = (double)p.adv[p.ag.offset(r)];
-  const double ratio = exp(lp - (double)p.old[p.og.offset(r)]);
-  const double lo = (double)p.low, hi = (double)p.high;
-  const bool inside = a > 0.0 ? ratio <= hi : ratio >= lo;
-  const double clipped = fmin(fmax(ratio, lo), hi);
-  term = fmax(-a * ratio, -a * clipped);
-  coef = inside ? -a * ratio : 0.0;
-  if (p.ref != nullptr) {
-    const double g = (double)p.ref[p.rg.offset(r)] - lp;
-    const double eg = expm1(g);
-    term += (double)p.kl * (eg - g);
-    coef -= (double)p.kl * eg;
+// What a row's loss term takes besides its log-probability.
+struct PolicyRow {
+  float old, adv, ref;
+  double weight;
+  __device__ __forceinline__ void load(const PolicyTerms& p, int64_t r, int64_t inner) {
+    old = p.old[p.og.offset(r)];
+    adv = p.adv[p.ag.offset(r)];
+    ref = p.ref != nullptr ? p.ref[p.rg.offset(r)] : 0.0f;
+    weight = p.weight[r / inner];
   }
-  term *= w;
-  coef *= w;
-}
+  // max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
+  // derivative to lp: -A r where the unclipped term is the larger one, and kl (1 - e^g). The
+  // differences are taken in 64 bits, the exponentials of these small numbers in 32.
+  __device__ __forceinline__ void term(const PolicyTerms& p, double lp, double& term,
+                                       float& coef) const {
+    const float r = expf((float)(lp - (double)old));
+    const bool inside = adv > 0.0f ? r <= p.high : r >= p.low;
+    const float gain = -adv * r;
+    double value = fmaxf(gain, -adv * fminf(fmaxf(r, p.low), p.high));
+    double slope = inside ? gain : 0.0f;
+    if (p.ref != nullptr) {
+      const double g = (double)ref - lp;
+      const float eg = expm1f((float)g);
+      value += (double)p.kl * ((double)eg - g);
+      slope -= (double)p.kl * (double)eg;
+    }
+    term = value * weight;
+    coef = (float)(slope * weight);
+  }
+};
 
 // Loss terms and coefficients of every row from the log-probabilities, one thread per row.
 __global__ void __launch_bounds__(kThreads)
 policy_row_kernel(const double* __restrict__ logps, Targets tg, int64_t rows, PolicyTerms p) {
   for (int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x; r < rows;
        r += (int64_t)gridDim.x * kThreads) {
-    double term = 0.0, coef = 0.0;
-    if (tg.at(r) != tg.ignore)
-      policy_term(p, r, logps[r], p.weight[r / tg.g.inner], term, coef);
+    double term = 0.0;
+    float coef = 0.0f;
+    if (tg.at(r) != tg.ignore) {
+      PolicyRow row;
+      row.load(p, r, tg.g.inner);
+      row.term(p, logps[r], term, coef);
+    }
     p.term[r] = term;
-    p.coef[r] = (float)coef;
+    p.coef[r] = coef;
   }
 }
 
@@ -480,6 +526,238 @@ policy_sum_kernel(const double* __restrict__ term, int64_t rows, const double* _
   s = block_sum(s, red);
   w = block_sum(w, red);
   if (threadIdx.x == 0) *loss = w > 0.0 ? (float)s : NAN;
+}
+
+// One pass for the loss and its gradient (see pt_policy_loss_grad): the coefficient of a row
+// depends on that row alone, so a row is read from HBM once, kept in shared memory while its
+// statistics form, and turned into dx from there: one read and one write of the logits' size
+// where the two-kernel form reads twice.
+//
+// A cluster of C CTAs takes one row, each a slice of whole 16-byte vectors. Every warp fetches
+// its own piece of the slice by one bulk copy, sums it when it has arrived and later turns the
+// same piece into dx, so warps meet only to merge their sums. The CTAs exchange theirs by
+// asynchronous stores into each other's shared memory, which complete on the receiver's barrier:
+// one thread waits for it, not the whole cluster. Several clusters share an SM, so one row's
+// loads overlap another's arithmetic and stores.
+#ifndef PT_POLICY_BLOCKS
+#define PT_POLICY_BLOCKS 4
+#endif
+#ifndef PT_POLICY_THREADS
+#define PT_POLICY_THREADS 256
+#endif
+#ifndef PT_POLICY_SLICE
+#define PT_POLICY_SLICE 32
+#endif
+constexpr int kFusedThreads = PT_POLICY_THREADS;
+constexpr int kFusedWarps = kFusedThreads / 32;
+constexpr int kMaxCluster = 8;  // the portable cluster size
+constexpr int kSliceBytes = PT_POLICY_SLICE * 1024;
+constexpr int kMaxSliceBytes = 192 * 1024;
+constexpr int kErrWait = kDeviceErrWaitTimeout;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cluster(const void* p, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(p)),
+               "r"(rank));
+  return remote;
+}
+// Stores v at the place that `p` (in this CTA's shared memory) has in CTA `rank`, counted by the
+// barrier that `bar` is there.
+__device__ __forceinline__ void store_in_cluster(Stat* p, uint64_t* bar, uint32_t rank, Stat v) {
+  asm volatile(
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::
+          "r"(in_cluster(p, rank)),
+      "r"(__float_as_uint(v.m)), "r"(__float_as_uint(v.s)), "r"(in_cluster(bar, rank))
+      : "memory");
+}
+// mbar_wait_bounded for data that other CTAs of the cluster have stored.
+__device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_addr(bar))
+        : "memory");
+    if (done) return true;
+    if (clock64() - t0 > kWaitLimitCycles) return false;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFusedThreads, PT_POLICY_BLOCKS)
+policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t vocab,
+                   int cluster, PolicyTerms p, float grad, RowOut out, T* __restrict__ dlogits,
+                   RowGrid dg) {
+  constexpr int V = Vec16<T>::N;
+  extern __shared__ __align__(16) unsigned char slice[];
+  __shared__ uint64_t bar[kFusedWarps];
+  __shared__ uint64_t peer_bar;
+  __shared__ Stat red[kFusedWarps];
+  __shared__ Stat peer[kMaxCluster];
+  __shared__ float3 shared_row;  // reference, 1 / s, coefficient
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+  const int64_t r = blockIdx.x / (unsigned)cluster;
+  const T* row = logits + lg.offset(r);
+  T* drow = dlogits + dg.offset(r);
+  const int64_t t = tg.at(r);
+  const RowKind kind = row_kind(t, tg.ignore, vocab);
+  const int head = head_elems(row, vocab);
+  const int64_t nvec = (vocab - head) / V;
+  const int64_t tail = head + nvec * V;
+  const Part part(nvec, rank, cluster);
+  const int n = (int)(part.v1 - part.v0);
+  const T* body = row + head + part.v0 * V;
+  T* dbody = drow + head + part.v0 * V;
+  // This thread's element of the unaligned head or tail, or -1.
+  int64_t edge = -1;
+  if (rank == 0 && tid < head) edge = tid;
+  if (rank == cluster - 1 && tid >= 32 && tail + tid - 32 < vocab) edge = tail + tid - 32;
+
+  if (kind != kRowUsed) {  // the same for every CTA of the cluster: none waits for another
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    for (int v = tid; v < n; v += kFusedThreads) st_stream(dbody + (int64_t)v * V, z);
+    if (edge >= 0) drow[edge] = from_float<T>(0.0f);
+    if (rank == 0 && tid == 0) {
+      out.store(r, kind, Stat{0.0f, 1.0f}, 0.0f);
+      p.term[r] = kind == kRowIgnored ? 0.0 : NAN;
+      p.coef[r] = 0.0f;
+    }
+    return;
+  }
+
+  const int per_warp = (n + kFusedWarps - 1) / kFusedWarps;
+  const int w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
+  if (lane == 0 && w1 > w0) {
+    mbar_init(&bar[warp], 1);
+    fence_mbar_init();
+    mbar_arrive_expect_tx(&bar[warp], (uint32_t)(w1 - w0) * 16u);
+    bulk_load(slice + (size_t)w0 * 16, body + (int64_t)w0 * V, (uint32_t)(w1 - w0) * 16u,
+              &bar[warp]);
+  }
+  if (cluster > 1) {
+    if (tid == 0) {
+      mbar_init(&peer_bar, 1);
+      fence_mbar_init();
+      mbar_arrive_expect_tx(&peer_bar, (uint32_t)(cluster * sizeof(Stat)));
+    }
+    // Says that this CTA runs and its barrier is set (which the fence above has published). All
+    // threads arrive here and wait below, each warp as one: the barrier counts warps.
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
+  float xt = 0.0f;
+  PolicyRow terms;
+  if (tid == 0) {
+    xt = to_float(row[t]);
+    terms.load(p, r, tg.g.inner);
+  }
+  const float xe = edge >= 0 ? to_float(row[edge]) : 0.0f;
+  Running acc;
+  if (edge >= 0) acc.add1(xe);
+  __syncwarp();
+  if (w1 > w0 && !mbar_wait_bounded(&bar[warp], 0) && lane == 0)
+    atomicExch(&g_logit_loss_error, kErrWait);
+  // Two vectors a trip, each with its own sums: twice the independent additions.
+  Running acc2;
+  int v = w0 + lane;
+  for (; v + 32 < w1; v += 64) {
+    float x[V], y[V];
+    unpack<T>(lds128(slice + (size_t)v * 16), x);
+    unpack<T>(lds128(slice + (size_t)(v + 32) * 16), y);
+    acc.template add<V>(x);
+    acc2.template add<V>(y);
+  }
+  if (v < w1) {
+    float x[V];
+    unpack<T>(lds128(slice + (size_t)v * 16), x);
+    acc.template add<V>(x);
+  }
+  if (cluster > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  const Stat s1 = acc.stat(), s2 = acc2.stat();
+  const float both = fmaxf(s1.m, s2.m);
+  Stat total = block_merge(Stat{both, sum_at(s1, both) + sum_at(s2, both)}, red);
+  if (cluster > 1 && tid < cluster) store_in_cluster(&peer[rank], &peer_bar, tid, total);
+  if (tid == 0) {
+    if (cluster > 1) {
+      // All CTAs' stores have arrived after this: none reaches into a CTA that has ended.
+      if (!cluster_wait_bounded(&peer_bar)) atomicExch(&g_logit_loss_error, kErrWait);
+      total = Stat{-INFINITY, 0.0f};
+      for (int c = 0; c < cluster; ++c) total.m = fmaxf(total.m, peer[c].m);
+      for (int c = 0; c < cluster; ++c) total.s += sum_at(peer[c], total.m);
+    }
+    double term;
+    float coef;
+    terms.term(p, log_softmax(total, xt), term, coef);
+    shared_row = make_float3(total.m, 1.0f / total.s, coef * grad);
+    if (rank == 0) {
+      out.store(r, kind, total, xt);
+      p.term[r] = term;
+      p.coef[r] = coef;
+    }
+  }
+  __syncthreads();
+  const float c = shared_row.z, a = -c * shared_row.y, nm = -shared_row.x;
+  auto one = [&](int64_t col, float x) {
+    const float e = fast_exp(x + nm);
+    drow[col] = from_float<T>(col == t ? fmaf(a, e, c) : a * e);
+  };
+  if (edge >= 0) one(edge, xe);
+  const float2 nm2 = splat2(nm), a2 = splat2(a);
+  // The target's vector in this slice, if it is here.
+  const int64_t from = t - (head + part.v0 * V);
+  const int tv = from >= 0 && from < (int64_t)n * V ? (int)(from / V) : -1;
+#pragma unroll 2
+  for (int u = w0 + lane; u < w1; u += 32) {
+    float x[V];
+    unpack<T>(lds128(slice + (size_t)u * 16), x);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 y = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2));
+      const float2 d = __fmul2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), a2);
+      x[e] = d.x;
+      x[e + 1] = d.y;
+    }
+    st_stream(dbody + (int64_t)u * V, pack<T>(x));
+    if (u == tv) one(t, to_float(row[t]));
+  }
+}
+
+// dx *= grad / expected, unless they are equal.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+rescale_kernel(T* __restrict__ dlogits, RowGrid dg, int64_t rows, int64_t vocab,
+               const float* __restrict__ grad, float expected) {
+  constexpr int V = Vec16<T>::N;
+  if (*grad == expected) return;
+  const float f = *grad / expected;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    T* row = dlogits + dg.offset(r);
+    const int head = head_elems(row, vocab);
+    const int64_t nvec = (vocab - head) / V;
+    for (int64_t v = threadIdx.x; v < nvec; v += kThreads) {
+      uint4* at = reinterpret_cast<uint4*>(row + head + v * V);
+      float x[V];
+      unpack<T>(*at, x);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] *= f;
+      *at = pack<T>(x);
+    }
+    if ((int)threadIdx.x < head) row[threadIdx.x] = from_float<T>(to_float(row[threadIdx.x]) * f);
+    for (int64_t c = head + nvec * V + threadIdx.x; c < vocab; c += kThreads)
+      row[c] = from_float<T>(to_float(row[c]) * f);
+  }
 }
 
 // ------------------------------------------------------------------------- host side --
@@ -567,12 +845,14 @@ int take_workspace(Workspace& w, const Rows& g, void* workspace, int64_t bytes) 
 int grid_of(int64_t items, int sms, int per_sm) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(items, (int64_t)sms * per_sm));
 }
+// One CTA per item, handed out as CTAs finish (items differ in length).
+int grid_of(int64_t items) { return (int)std::min<int64_t>(items, INT32_MAX); }
 
 template <typename T>
 void launch_stats(const Rows& g, const void* logits, Stat* part, const RowOut& out,
                   cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
-  stats_kernel<T><<<grid_of(g.rows * g.splits, g.sms, 2048 / kThreads), kThreads, 0, s>>>(
+  stats_kernel<T><<<grid_of(g.rows * g.splits), kThreads, 0, s>>>(
       x, g.lg, g.tg, g.rows, g.vocab, g.splits, part, out);
   if (g.splits > 1)
     finish_kernel<T><<<grid_of((g.rows + 3) / 4, g.sms, 2048 / kThreads), kThreads, 0, s>>>(
@@ -587,6 +867,108 @@ void row_stats(const Rows& g, const void* logits, int dtype, Stat* part, const R
     case PT_FLOAT16: return launch_stats<__half>(g, logits, part, out, s);
     default: return launch_stats<__nv_bfloat16>(g, logits, part, out, s);
   }
+}
+
+// Rows of logits and of their gradient have to start at the same place of a 16-byte vector.
+int check_same_rows(const Rows& g, const void* logits, int64_t lo, int64_t li, const void* dlogits,
+                    int64_t dlo, int64_t dli, int elem) {
+  const uintptr_t gap = reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits);
+  if (gap % 16 || (g.outer > 1 && (lo - dlo) * elem % 16) ||
+      (g.inner > 1 && (li - dli) * elem % 16))
+    return set_error(PT_ERR_SHAPE, "rows of logits and dlogits must have the same address modulo "
+                                   "16 bytes");
+  return PT_OK;
+}
+
+struct PolicyInputs {
+  const float* old;
+  int64_t oo, oi;
+  const float* adv;
+  int64_t ao, ai;
+  const float* ref;
+  int64_t ro, ri;
+  double low, high, kl;
+};
+
+int check_policy(Rows& g, Workspace& w, PolicyTerms& p, const PolicyInputs& in,
+                 const void* logits, int64_t vocab, int64_t outer, int64_t inner, int64_t lo,
+                 int64_t li, const int64_t* targets, int64_t to, int64_t ti, int64_t ignore,
+                 float* loss, float* logps, float* stats, float* coef, void* workspace,
+                 int64_t workspace_size, int dtype) {
+  if (!(in.low >= 0.0) || !(in.high >= 0.0) || !std::isfinite(in.kl))
+    return set_error(PT_ERR_INVALID_ARGUMENT,
+                     "clip_low and clip_high must be >= 0 and kl_coef finite");
+  if (int st = check_rows(g, logits, vocab, outer, inner, lo, li, targets, to, ti, ignore, dtype))
+    return st;
+  if (int st = check_device_ptr(loss, "loss")) return st;
+  if (int st = check_optional(in.old, "old_logps", g.rows)) return st;
+  if (int st = check_optional(in.adv, "advantages", g.rows)) return st;
+  if (in.ref)
+    if (int st = check_optional(in.ref, "reference", g.rows)) return st;
+  if (int st = check_optional(logps, "logps", g.rows)) return st;
+  if (int st = check_optional(stats, "stats", g.rows)) return st;
+  if (int st = check_optional(coef, "coef", g.rows)) return st;
+  if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
+  p.old = in.old;
+  p.og = RowGrid{g.inner, in.oo, in.oi};
+  p.adv = in.adv;
+  p.ag = RowGrid{g.inner, in.ao, in.ai};
+  p.ref = in.ref;
+  p.rg = RowGrid{g.inner, in.ro, in.ri};
+  p.weight = w.seq;
+  p.low = (float)(1.0 - in.low);
+  p.high = (float)(1.0 + in.high);
+  p.kl = (float)in.kl;
+  p.term = w.term;
+  p.coef = coef;
+  return PT_OK;
+}
+
+// CTAs per row of the one-pass policy loss: as few as keep a slice within kSliceBytes, more (down
+// to 4 KB a slice) while the rows alone do not give every SM eight CTAs; larger slices where
+// the row does not fit eight such, 0 where it does not fit at all.
+int cluster_size(int64_t rows, int64_t row_bytes, int sms) {
+  if (row_bytes > (int64_t)kMaxCluster * kMaxSliceBytes || rows > INT32_MAX / kMaxCluster) return 0;
+  int c = 1;
+  while (c < kMaxCluster && (row_bytes > (int64_t)c * kSliceBytes ||
+                             (rows * c < (int64_t)sms * 8 && row_bytes >= (int64_t)c * 8192)))
+    c *= 2;
+  return c;
+}
+
+template <typename T>
+int launch_policy_grad(const Rows& g, const void* logits, int cluster, const PolicyTerms& p,
+                       float grad, const RowOut& out, void* dlogits, const RowGrid& dg,
+                       cudaStream_t s) {
+  // The largest slice: ceil(vectors / cluster) vectors (an unaligned row has fewer whole ones).
+  const int64_t nvec = g.vocab / Vec16<T>::N;
+  const size_t smem = (size_t)((nvec + cluster - 1) / cluster) * 16;
+  // The limit is the same on every call: calls on two threads must not lower each other's.
+  cudaError_t e = cudaFuncSetAttribute(policy_grad_kernel<T>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kMaxSliceBytes);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(g.rows * cluster));
+    cfg.blockDim = dim3(kFusedThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, policy_grad_kernel<T>, static_cast<const T*>(logits), g.lg, g.tg,
+                           g.vocab, cluster, p, grad, out, static_cast<T*>(dlogits), dg);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(PT_ERR_CUDA, "pt_policy_loss_grad: launch failed: %s",
+                     cudaGetErrorString(e));
+  }
+  return PT_OK;
 }
 
 }  // namespace
@@ -662,33 +1044,31 @@ int pt_token_logps_bwd(const void* logits, int64_t vocab, int64_t outer, int64_t
   if (int st = check_device_ptr(dlogits, "dlogits")) return st;
   if (grad)
     if (int st = check_device_ptr(grad, "grad")) return st;
-  const int elem = dtype_size(dtype);
-  const bool same = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) %
-                            16 == 0 &&
-                    (outer < 2 || (logits_outer_stride - dlogits_outer_stride) * elem % 16 == 0) &&
-                    (inner < 2 || (logits_inner_stride - dlogits_inner_stride) * elem % 16 == 0);
-  if (!same)
-    return set_error(PT_ERR_SHAPE, "rows of logits and dlogits must have the same address modulo "
-                                   "16 bytes");
+  if (int st = check_same_rows(g, logits, logits_outer_stride, logits_inner_stride, dlogits,
+                               dlogits_outer_stride, dlogits_inner_stride, dtype_size(dtype)))
+    return st;
   const RowGrid cg{g.inner, coef_outer_stride, coef_inner_stride};
   const RowGrid dg{g.inner, dlogits_outer_stride, dlogits_inner_stride};
   const float2* st2 = reinterpret_cast<const float2*>(stats);
-  const int grid = grid_of(g.rows * g.splits, g.sms, 2048 / kThreads);
+  const int64_t vecs = vocab * dtype_size(dtype) / 16;
+  const int splits =
+      (int)std::max<int64_t>(1, vecs / (kThreads * kUnrollGrad * kGradTrips));
+  const int grid = grid_of(g.rows * splits);
   cudaStream_t s = as_stream(stream);
   switch (dtype) {
     case PT_FLOAT32:
       grad_kernel<float><<<grid, kThreads, 0, s>>>(static_cast<const float*>(logits), g.lg, g.tg,
-                                                   g.rows, vocab, g.splits, st2, coef, cg, grad,
+                                                   g.rows, vocab, splits, st2, coef, cg, grad,
                                                    static_cast<float*>(dlogits), dg);
       break;
     case PT_FLOAT16:
       grad_kernel<__half><<<grid, kThreads, 0, s>>>(static_cast<const __half*>(logits), g.lg,
-                                                    g.tg, g.rows, vocab, g.splits, st2, coef, cg,
+                                                    g.tg, g.rows, vocab, splits, st2, coef, cg,
                                                     grad, static_cast<__half*>(dlogits), dg);
       break;
     default:
       grad_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(
-          static_cast<const __nv_bfloat16*>(logits), g.lg, g.tg, g.rows, vocab, g.splits, st2,
+          static_cast<const __nv_bfloat16*>(logits), g.lg, g.tg, g.rows, vocab, splits, st2,
           coef, cg, grad, static_cast<__nv_bfloat16*>(dlogits), dg);
   }
   return check_launch("pt_token_logps_bwd");
@@ -748,37 +1128,18 @@ int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t
                        float* loss, float* logps, float* stats, float* coef, void* workspace,
                        int64_t workspace_size, int dtype, void* stream) {
   Rows g;
-  if (!(clip_low >= 0.0) || !(clip_high >= 0.0) || !std::isfinite(kl_coef))
-    return set_error(PT_ERR_INVALID_ARGUMENT,
-                     "clip_low and clip_high must be >= 0 and kl_coef finite");
-  if (int st = check_rows(g, logits, vocab, outer, inner, logits_outer_stride,
-                          logits_inner_stride, targets, targets_outer_stride,
-                          targets_inner_stride, ignore_index, dtype))
-    return st;
-  if (int st = check_device_ptr(loss, "loss")) return st;
-  if (int st = check_optional(old_logps, "old_logps", g.rows)) return st;
-  if (int st = check_optional(advantages, "advantages", g.rows)) return st;
-  if (reference)
-    if (int st = check_optional(reference, "reference", g.rows)) return st;
-  if (int st = check_optional(logps, "logps", g.rows)) return st;
-  if (int st = check_optional(stats, "stats", g.rows)) return st;
-  if (int st = check_optional(coef, "coef", g.rows)) return st;
   Workspace w;
-  if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
-  cudaStream_t s = as_stream(stream);
   PolicyTerms p;
-  p.old = old_logps;
-  p.og = RowGrid{g.inner, old_outer_stride, old_inner_stride};
-  p.adv = advantages;
-  p.ag = RowGrid{g.inner, advantages_outer_stride, advantages_inner_stride};
-  p.ref = reference;
-  p.rg = RowGrid{g.inner, reference_outer_stride, reference_inner_stride};
-  p.weight = w.seq;
-  p.low = (float)(1.0 - clip_low);
-  p.high = (float)(1.0 + clip_high);
-  p.kl = (float)kl_coef;
-  p.term = w.term;
-  p.coef = coef;
+  const PolicyInputs in{old_logps, old_outer_stride, old_inner_stride,
+                        advantages, advantages_outer_stride, advantages_inner_stride,
+                        reference, reference_outer_stride, reference_inner_stride,
+                        clip_low, clip_high, kl_coef};
+  if (int st = check_policy(g, w, p, in, logits, vocab, outer, inner, logits_outer_stride,
+                            logits_inner_stride, targets, targets_outer_stride,
+                            targets_inner_stride, ignore_index, loss, logps, stats, coef,
+                            workspace, workspace_size, dtype))
+    return st;
+  cudaStream_t s = as_stream(stream);
   row_stats(g, logits, dtype, w.part, RowOut{reinterpret_cast<float2*>(stats), logps, w.logps},
             s);
   const int64_t sequences = g.rows > 0 ? outer : 0;
@@ -788,6 +1149,107 @@ int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t
                         kThreads, 0, s>>>(w.logps, g.tg, g.rows, p);
   policy_sum_kernel<<<1, kSumThreads, 0, s>>>(w.term, g.rows, w.seq, sequences, loss);
   return check_launch("pt_policy_loss_fwd");
+}
+
+int pt_policy_loss_grad_supported(int64_t vocab, int64_t outer, int64_t inner, int dtype,
+                                  int* supported) {
+  if (supported == nullptr) return set_error(PT_ERR_INVALID_ARGUMENT, "supported is NULL");
+  int64_t rows = 0;
+  if (int st = check_sizes(vocab, outer, inner, &rows)) return st;
+  const int elem = dtype_size(dtype);
+  if (elem == 0) return set_error(PT_ERR_UNSUPPORTED_DTYPE, "unsupported dtype %d", dtype);
+  *supported = cluster_size(rows, vocab * elem, 1) > 0;
+  return ok();
+}
+
+int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
+                        int64_t logits_outer_stride, int64_t logits_inner_stride,
+                        const int64_t* targets, int64_t targets_outer_stride,
+                        int64_t targets_inner_stride, int64_t ignore_index,
+                        const float* old_logps, int64_t old_outer_stride, int64_t old_inner_stride,
+                        const float* advantages, int64_t advantages_outer_stride,
+                        int64_t advantages_inner_stride, const float* reference,
+                        int64_t reference_outer_stride, int64_t reference_inner_stride,
+                        double clip_low, double clip_high, double kl_coef, int by_sequence,
+                        double grad, float* loss, float* logps, float* stats, float* coef,
+                        void* dlogits, int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
+                        void* workspace, int64_t workspace_size, int dtype, void* stream) {
+  Rows g;
+  Workspace w;
+  PolicyTerms p;
+  const PolicyInputs in{old_logps, old_outer_stride, old_inner_stride,
+                        advantages, advantages_outer_stride, advantages_inner_stride,
+                        reference, reference_outer_stride, reference_inner_stride,
+                        clip_low, clip_high, kl_coef};
+  if (int st = check_policy(g, w, p, in, logits, vocab, outer, inner, logits_outer_stride,
+                            logits_inner_stride, targets, targets_outer_stride,
+                            targets_inner_stride, ignore_index, loss, logps, stats, coef,
+                            workspace, workspace_size, dtype))
+    return st;
+  if (int st = check_optional(dlogits, "dlogits", g.rows)) return st;
+  if (g.rows > 0)
+    if (int st = check_same_rows(g, logits, logits_outer_stride, logits_inner_stride, dlogits,
+                                 dlogits_outer_stride, dlogits_inner_stride, dtype_size(dtype)))
+      return st;
+  const int cluster = cluster_size(g.rows, vocab * dtype_size(dtype), g.sms);
+  if (cluster == 0)
+    return set_error(PT_ERR_SHAPE, "rows of %lld logits do not fit on chip (or too many rows)",
+                     (long long)vocab);
+  cudaStream_t s = as_stream(stream);
+  const int64_t sequences = g.rows > 0 ? outer : 0;
+  policy_weight_kernel<<<1, kSumThreads, 0, s>>>(g.tg, sequences, by_sequence, w.seq);
+  if (g.rows > 0) {
+    const RowGrid dg{g.inner, dlogits_outer_stride, dlogits_inner_stride};
+    const RowOut out{reinterpret_cast<float2*>(stats), logps, nullptr};
+    int st;
+    switch (dtype) {
+      case PT_FLOAT32:
+        st = launch_policy_grad<float>(g, logits, cluster, p, (float)grad, out, dlogits, dg, s);
+        break;
+      case PT_FLOAT16:
+        st = launch_policy_grad<__half>(g, logits, cluster, p, (float)grad, out, dlogits, dg, s);
+        break;
+      default:
+        st = launch_policy_grad<__nv_bfloat16>(g, logits, cluster, p, (float)grad, out, dlogits,
+                                               dg, s);
+    }
+    if (st) return st;
+  }
+  policy_sum_kernel<<<1, kSumThreads, 0, s>>>(w.term, g.rows, w.seq, sequences, loss);
+  return check_launch("pt_policy_loss_grad");
+}
+
+int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t inner,
+                           int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
+                           const float* grad, double expected, int dtype, void* stream) {
+  int64_t rows = 0;
+  if (int st = check_sizes(vocab, outer, inner, &rows)) return st;
+  if (dtype_size(dtype) == 0)
+    return set_error(PT_ERR_UNSUPPORTED_DTYPE, "unsupported dtype %d", dtype);
+  if (!std::isfinite(expected) || expected == 0.0)
+    return set_error(PT_ERR_INVALID_ARGUMENT, "expected must be finite and not 0");
+  if (rows == 0) return ok();
+  if (int st = check_device_ptr(dlogits, "dlogits")) return st;
+  if (int st = check_device_ptr(grad, "grad")) return st;
+  int sms = 0;
+  if (int st = current_device_info(nullptr, &sms)) return st;
+  const RowGrid dg{inner, dlogits_outer_stride, dlogits_inner_stride};
+  const int grid = grid_of(rows, sms, 2048 / kThreads);
+  cudaStream_t s = as_stream(stream);
+  switch (dtype) {
+    case PT_FLOAT32:
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<float*>(dlogits), dg, rows, vocab, grad,
+                                               (float)expected);
+      break;
+    case PT_FLOAT16:
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__half*>(dlogits), dg, rows, vocab,
+                                               grad, (float)expected);
+      break;
+    default:
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__nv_bfloat16*>(dlogits), dg, rows,
+                                               vocab, grad, (float)expected);
+  }
+  return check_launch("pt_rescale_logits_grad");
 }
 
 }  // extern "C"

@@ -19,9 +19,12 @@ word (a kernel cannot raise). Calls that cannot run raise
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor
 
+from picotron_b200 import ops
 from picotron_b200.errors import TritonLogitLossUnavailable
 
 
@@ -50,7 +53,7 @@ def token_log_probs(logits: Tensor, targets: Tensor, *, ignore_index: int = -100
     """
 
     _check_tensors(logits=logits, targets=targets)
-    return torch.ops.picotron_b200.token_logps(logits, targets, int(ignore_index))[0]
+    return ops.token_logps(logits, targets, int(ignore_index))[0]
 
 
 def preference_loss(logits: Tensor, targets: Tensor, reference_log_probs: Tensor, *,
@@ -70,15 +73,16 @@ def preference_loss(logits: Tensor, targets: Tensor, reference_log_probs: Tensor
 
     _check_tensors(logits=logits, targets=targets, reference_log_probs=reference_log_probs)
     reference = _per_token(reference_log_probs, targets, "reference_log_probs")
-    loss, rewards, _, _ = torch.ops.picotron_b200.preference_loss(
+    loss, rewards, _, _ = ops.preference_loss(
         logits, targets, reference, float(beta), float(label_smoothing), int(ignore_index))
-    return loss, rewards.detach()
+    return loss, rewards
 
 
 def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantages: Tensor, *,
                 reference_log_probs: Tensor | None = None, kl_coef: float = 0.0,
                 clip_low: float = 0.2, clip_high: float = 0.2, aggregate: str = "token",
-                ignore_index: int = -100) -> tuple[Tensor, Tensor]:
+                ignore_index: int = -100,
+                expected_grad: float | None = None) -> tuple[Tensor, Tensor]:
     """Clipped policy-gradient loss with a KL term; returns ``(loss, log_probs)``.
 
     With ``r = exp(log_probs - old_log_probs)``, ``A = advantages`` ([B], one per sequence, or
@@ -91,6 +95,14 @@ def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantag
     target, ``"sequence"`` over the means of the sequences that have any; the loss is NaN when
     there are none. ``log_probs`` is shaped like ``targets`` (0 where ignored) and carries no
     gradient.
+
+    Where the logits need a gradient it is formed with the loss, in one pass over them, for the
+    gradient that the loss is expected to receive; ``backward`` then only compares. That is 1 by
+    default (``loss.backward()``); give ``expected_grad`` where the loss is scaled before it, e.g.
+    ``1 / steps`` for ``(loss / steps).backward()`` or a loss scaler's scale. Any other gradient
+    is still right but costs a pass to rescale, and rounds the result once more. float16 logits
+    form their gradient in ``backward`` unless ``expected_grad`` is given, since it would
+    underflow without the loss scale.
     """
 
     _check_tensors(logits=logits, targets=targets, old_log_probs=old_log_probs,
@@ -98,6 +110,8 @@ def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantag
     if aggregate not in ("token", "sequence"):
         raise TritonLogitLossUnavailable(
             f'aggregate must be "token" or "sequence", not {aggregate!r}')
+    if expected_grad is not None and not (math.isfinite(expected_grad) and expected_grad != 0):
+        raise TritonLogitLossUnavailable("expected_grad must be finite and not 0.")
     reference = None
     if kl_coef != 0.0:
         if reference_log_probs is None:
@@ -106,8 +120,9 @@ def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantag
         reference = _per_token(reference_log_probs, targets, "reference_log_probs")
     if targets.dim() == 2 and advantages.shape == targets.shape[:1]:
         advantages = advantages[:, None].expand(targets.shape)
-    loss, log_probs, _, _ = torch.ops.picotron_b200.policy_loss(
+    loss, log_probs, _, _ = ops.policy_loss(
         logits, targets, _per_token(old_log_probs, targets, "old_log_probs"),
         _per_token(advantages, targets, "advantages"), reference, float(clip_low),
-        float(clip_high), float(kl_coef), aggregate == "sequence", int(ignore_index))
-    return loss, log_probs.detach()
+        float(clip_high), float(kl_coef), aggregate == "sequence", int(ignore_index),
+        None if expected_grad is None else float(expected_grad))
+    return loss, log_probs

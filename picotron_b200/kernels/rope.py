@@ -124,5 +124,4 @@ def apply_rotary_positions(query: Tensor, key: Tensor, positions: Tensor, inv_fr
             raise TritonRoPEUnavailable("sm_100a RoPE requires CUDA tensors.")
     if layout not in ops.LAYOUTS:
         raise TritonRoPEUnavailable(f"unknown RoPE layout {layout!r}")
-    return torch.ops.picotron_b200.rope_positions(query, key, positions, inv_freq,
-                                                  ops.LAYOUTS[layout], float(scale))
+    return ops.rope_positions(query, key, positions, inv_freq, ops.LAYOUTS[layout], float(scale))

@@ -649,6 +649,40 @@ def _ce_backward(ctx, grad, _grad_lse, _grad_mean):
 cross_entropy.register_autograd(_ce_backward, setup_context=_ce_setup)
 
 
+# The ops below are registered through torch.library.Library with an autograd.Function each,
+# where those above use custom_op: the same torch.ops.picotron_b200 entries and fake
+# implementations, but a forward + backward call costs 42 us of host time instead of 148
+# (measured without kernels), which is what a small call takes.
+
+_LIBRARY = torch.library.Library("picotron_b200", "FRAGMENT")
+
+
+def _register(schema: str, run, fake, function: type[torch.autograd.Function] | None = None):
+    """Define an op with its implementation (which checks the device itself), its fake one and, for
+    a differentiable op, the autograd Function to take where the first argument that may need
+    a gradient does; returns the op."""
+
+    name = schema.split("(")[0]
+    _LIBRARY.define(schema)
+    _LIBRARY.impl(name, run, "CompositeExplicitAutograd")
+    torch.library.register_fake(f"picotron_b200::{name}", fake, lib=_LIBRARY)
+    op = getattr(torch.ops.picotron_b200, name).default
+    if function is not None:
+        def autograd(*args):
+            if torch.is_grad_enabled() and any(
+                    isinstance(a, Tensor) and a.requires_grad for a in args):
+                return function.apply(*args)
+            return _below_autograd(op, *args)
+
+        _LIBRARY.impl(name, autograd, "Autograd")
+    return op
+
+
+def _below_autograd(op, *args):
+    with torch._C._AutoDispatchBelowAutograd():
+        return op(*args)
+
+
 # ------------------------------------------------------ losses over log-probabilities --
 
 
@@ -743,8 +777,7 @@ def _ll_gradient(logits: Tensor) -> Tensor:
     return buffer.as_strided(logits.shape, strides, shift)
 
 
-@torch.library.custom_op("picotron_b200::token_logps", mutates_args=())
-def token_logps(logits: Tensor, targets: Tensor, ignore_index: int) -> tuple[Tensor, Tensor]:
+def _token_logps(logits: Tensor, targets: Tensor, ignore_index: int) -> tuple[Tensor, Tensor]:
     x, outer, inner = _ll_inputs(logits, targets)
     logps = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
     stats = torch.empty((*targets.shape, 2), dtype=torch.float32, device=x.device)
@@ -759,15 +792,13 @@ def token_logps(logits: Tensor, targets: Tensor, ignore_index: int) -> tuple[Ten
     return logps, stats
 
 
-@token_logps.register_fake
 def _token_logps_fake(logits, targets, ignore_index):
     return (torch.empty(targets.shape, dtype=torch.float32, device=logits.device),
             torch.empty((*targets.shape, 2), dtype=torch.float32, device=logits.device))
 
 
-@torch.library.custom_op("picotron_b200::logit_loss_backward", mutates_args=())
-def logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: Tensor,
-                        grad: Tensor | None, ignore_index: int) -> Tensor:
+def _logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: Tensor,
+                         grad: Tensor | None, ignore_index: int) -> Tensor:
     """dlogits = coef * grad * (onehot(targets) - softmax(logits)); coef has the targets' shape
     (and any strides), grad is one value."""
 
@@ -788,7 +819,6 @@ def logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: Te
     return dlogits
 
 
-@logit_loss_backward.register_fake
 def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
     x = _ll_logits(logits)
     if _ll_dense_gradient(x):
@@ -796,27 +826,37 @@ def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
     return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
 
 
-def _token_logps_setup(ctx, inputs, output) -> None:
-    logits, targets, ctx.ignore_index = inputs
-    ctx.save_for_backward(logits, targets, output[1])
-    ctx.set_materialize_grads(False)
+logit_loss_backward = _register(
+    "logit_loss_backward(Tensor logits, Tensor targets, Tensor stats, Tensor coef, Tensor? grad, "
+    "int ignore_index) -> Tensor", _logit_loss_backward, _logit_loss_backward_fake)
 
 
-def _token_logps_bwd(ctx, grad, _grad_stats):
-    if grad is None:
-        return None, None, None
-    logits, targets, stats = ctx.saved_tensors
-    return torch.ops.picotron_b200.logit_loss_backward(logits, targets, stats, grad, None,
-                                                       ctx.ignore_index), None, None
+class _TokenLogps(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, ignore_index):
+        logps, stats = _below_autograd(token_logps, logits, targets, ignore_index)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
+        return logps, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _grad_stats):
+        if grad is None:
+            return None, None, None
+        return logit_loss_backward(*ctx.saved_tensors, grad, None, ctx.ignore_index), None, None
 
 
-token_logps.register_autograd(_token_logps_bwd, setup_context=_token_logps_setup)
+token_logps = _register(
+    "token_logps(Tensor logits, Tensor targets, int ignore_index) -> (Tensor, Tensor)",
+    _token_logps, _token_logps_fake, _TokenLogps)
 
 
-@torch.library.custom_op("picotron_b200::preference_loss", mutates_args=())
-def preference_loss(logits: Tensor, targets: Tensor, reference: Tensor, beta: float,
-                    label_smoothing: float,
-                    ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+def _preference_loss(logits: Tensor, targets: Tensor, reference: Tensor, beta: float,
+                     label_smoothing: float,
+                     ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(loss, rewards, stats, coef) of pt_preference_loss_fwd."""
 
     x, outer, inner = _ll_inputs(logits, targets, (reference,))
@@ -838,35 +878,45 @@ def preference_loss(logits: Tensor, targets: Tensor, reference: Tensor, beta: fl
     return loss, rewards, stats, coef
 
 
-@preference_loss.register_fake
 def _preference_loss_fake(logits, targets, reference, beta, label_smoothing, ignore_index):
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
     return new(), new(logits.size(0)), new(*targets.shape, 2), new(logits.size(0))
 
 
-def _preference_setup(ctx, inputs, output) -> None:
-    logits, targets, _, _, _, ctx.ignore_index = inputs
-    ctx.save_for_backward(logits, targets, output[2], output[3])
-    ctx.set_materialize_grads(False)
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, reference, beta, label_smoothing, ignore_index):
+        loss, *rest = _below_autograd(preference_loss, logits, targets, reference, beta,
+                                      label_smoothing, ignore_index)
+        rewards, stats, coef = rest
+        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(*rest)
+        ctx.set_materialize_grads(False)
+        return loss, rewards, stats, coef
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        if grad is None:
+            return (None,) * 6
+        logits, targets, stats, coef = ctx.saved_tensors
+        dlogits = logit_loss_backward(logits, targets, stats,
+                                      coef[:, None].expand(targets.shape), grad,
+                                      ctx.ignore_index)
+        return dlogits, None, None, None, None, None
 
 
-def _preference_bwd(ctx, grad, *_):
-    if grad is None:
-        return (None,) * 6
-    logits, targets, stats, coef = ctx.saved_tensors
-    dlogits = torch.ops.picotron_b200.logit_loss_backward(
-        logits, targets, stats, coef[:, None].expand(targets.shape), grad, ctx.ignore_index)
-    return dlogits, None, None, None, None, None
+preference_loss = _register(
+    "preference_loss(Tensor logits, Tensor targets, Tensor reference, float beta, "
+    "float label_smoothing, int ignore_index) -> (Tensor, Tensor, Tensor, Tensor)",
+    _preference_loss, _preference_loss_fake, _PreferenceLoss)
 
 
-preference_loss.register_autograd(_preference_bwd, setup_context=_preference_setup)
-
-
-@torch.library.custom_op("picotron_b200::policy_loss", mutates_args=())
-def policy_loss(logits: Tensor, targets: Tensor, old_logps: Tensor, advantages: Tensor,
-                reference: Tensor | None, clip_low: float, clip_high: float, kl_coef: float,
-                by_sequence: bool,
-                ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+def _policy_loss(logits: Tensor, targets: Tensor, old_logps: Tensor, advantages: Tensor,
+                 reference: Tensor | None, clip_low: float, clip_high: float, kl_coef: float,
+                 by_sequence: bool, ignore_index: int,
+                 expected_grad: float | None) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(loss, logps, stats, coef) of pt_policy_loss_fwd."""
 
     per_token = (old_logps, advantages) if reference is None else (old_logps, advantages, reference)
@@ -888,29 +938,107 @@ def policy_loss(logits: Tensor, targets: Tensor, old_logps: Tensor, advantages: 
     return loss, logps, stats, coef
 
 
-@policy_loss.register_fake
 def _policy_loss_fake(logits, targets, old_logps, advantages, reference, clip_low, clip_high,
-                      kl_coef, by_sequence, ignore_index):
+                      kl_coef, by_sequence, ignore_index, expected_grad=None):
     new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
     return new(), new(*targets.shape), new(*targets.shape, 2), new(*targets.shape)
 
 
-def _policy_setup(ctx, inputs, output) -> None:
-    ctx.ignore_index = inputs[-1]
-    ctx.save_for_backward(inputs[0], inputs[1], output[2], output[3])
-    ctx.set_materialize_grads(False)
+def _policy_loss_grad(logits, targets, old_logps, advantages, reference, clip_low, clip_high,
+                      kl_coef, by_sequence, ignore_index, grad):
+    """policy_loss's outputs and dlogits = grad * d loss / d logits, in one pass over the logits
+    (pt_policy_loss_grad)."""
+
+    per_token = (old_logps, advantages) if reference is None else (old_logps, advantages, reference)
+    x, outer, inner = _ll_inputs(logits, targets, per_token)
+    loss, logps, stats, coef = _policy_loss_fake(x, targets, old_logps, advantages, reference,
+                                                 clip_low, clip_high, kl_coef, by_sequence,
+                                                 ignore_index)
+    dlogits = _ll_gradient(x)
+    with _OnDevice(x.device):
+        work = _ll_workspace(x, outer, inner)
+        _capi.policy_loss_grad(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
+                               ignore_index, _ll_rows(old_logps), _ll_rows(advantages),
+                               _ll_rows(reference) if reference is not None else (None, 0, 0),
+                               clip_low, clip_high, kl_coef, by_sequence, grad, loss.data_ptr(),
+                               logps.data_ptr(), stats.data_ptr(), coef.data_ptr(),
+                               _ll_logits_rows(dlogits), work.data_ptr(), work.numel(),
+                               DTYPE_CODES[x.dtype], _stream(x.device),
+                               TritonLogitLossUnavailable)
+    return loss, logps, stats, coef, dlogits
 
 
-def _policy_bwd(ctx, grad, *_):
-    if grad is None:
-        return (None,) * 10
-    logits, targets, stats, coef = ctx.saved_tensors
-    dlogits = torch.ops.picotron_b200.logit_loss_backward(logits, targets, stats, coef, grad,
-                                                          ctx.ignore_index)
-    return (dlogits, *(None,) * 9)
+def _policy_loss_grad_fake(logits, targets, *args):
+    return (*_policy_loss_fake(logits, targets, *args[:-1]),
+            _logit_loss_backward_fake(logits, targets, None, None, None, None))
 
 
-policy_loss.register_autograd(_policy_bwd, setup_context=_policy_setup)
+def _one_pass_policy(logits: Tensor, targets: Tensor, expected: float | None) -> float | None:
+    """The factor to form the policy loss's gradient with in its forward, or None to form it in
+    the backward. Without a hint float16 waits: it is trained under a loss scale, without which
+    its gradients would underflow."""
+
+    if expected is None and logits.dtype != torch.float16:
+        expected = 1.0
+    # A traced graph (its tensors are subclasses) cannot carry the in-place rescaling and takes
+    # the two passes.
+    if expected is None or type(logits) not in (Tensor, torch.nn.Parameter):
+        return None
+    outer, inner = _ll_geometry(logits, targets)
+    code = _dtype_code(logits, TritonLogitLossUnavailable)
+    if logits.size(-1) < 1 or not _capi.policy_loss_grad_supported(
+            logits.size(-1), outer, inner, code, TritonLogitLossUnavailable):
+        return None
+    return expected
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, *args):
+        *args, expected = args
+        ctx.expected = _one_pass_policy(logits, targets, expected)
+        if ctx.expected is None:
+            loss, *rest = _below_autograd(policy_loss, logits, targets, *args, expected)
+            ctx.dlogits = None
+        else:
+            loss, *rest, ctx.dlogits = _below_autograd(policy_loss_grad, logits, targets, *args,
+                                                       ctx.expected)
+        logps, stats, coef = rest
+        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.ignore_index = args[-1]
+        ctx.mark_non_differentiable(*rest)
+        ctx.set_materialize_grads(False)
+        return loss, logps, stats, coef
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        if grad is None:
+            return (None,) * 11
+        logits, targets, stats, coef = ctx.saved_tensors
+        dlogits, ctx.dlogits = ctx.dlogits, None
+        if dlogits is None:  # two passes, or a second backward through a retained graph
+            dlogits = logit_loss_backward(logits, targets, stats, coef, grad, ctx.ignore_index)
+        elif dlogits.numel():
+            outer, inner = _ll_geometry(logits, targets)
+            grad = grad.to(torch.float32)
+            with _OnDevice(logits.device):
+                _capi.rescale_logits_grad(_ll_logits_rows(dlogits), dlogits.size(-1), outer,
+                                          inner, grad.data_ptr(), ctx.expected,
+                                          DTYPE_CODES[logits.dtype], _stream(logits.device),
+                                          TritonLogitLossUnavailable)
+        return dlogits, *(None,) * 10
+
+
+_POLICY = ("(Tensor logits, Tensor targets, Tensor old_logps, Tensor advantages, "
+           "Tensor? reference, float clip_low, float clip_high, float kl_coef, bool by_sequence, "
+           "int ignore_index, ")
+policy_loss_grad = _register(
+    f"policy_loss_grad{_POLICY}float grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    _policy_loss_grad, _policy_loss_grad_fake)
+policy_loss = _register(
+    f"policy_loss{_POLICY}float? expected_grad) -> (Tensor, Tensor, Tensor, Tensor)",
+    _policy_loss, _policy_loss_fake, _PolicyLoss)
 
 
 # ------------------------------------------------------------------------------ RoPE --
@@ -1121,15 +1249,11 @@ def _rope_state(x: Tensor) -> tuple[Tensor, Tensor]:
     return x, out if out.stride(-1) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-@torch.library.custom_op("picotron_b200::rope_positions", mutates_args=())
-def rope_positions(q: Tensor, k: Tensor, positions: Tensor, inv_freq: Tensor, layout: int,
-                   scale: float) -> tuple[Tensor, Tensor]:
+def _rope_positions(q, k, positions, inv_freq, layout, scale):
     return _rope_positions_launch(False, q, k, positions, inv_freq, layout, scale)
 
 
-@torch.library.custom_op("picotron_b200::rope_positions_backward", mutates_args=())
-def rope_positions_backward(dq: Tensor, dk: Tensor, positions: Tensor, inv_freq: Tensor,
-                            layout: int, scale: float) -> tuple[Tensor, Tensor]:
+def _rope_positions_backward(dq, dk, positions, inv_freq, layout, scale):
     return _rope_positions_launch(True, dq, dk, positions, inv_freq, layout, scale)
 
 
@@ -1137,27 +1261,27 @@ def _rope_positions_fake(q, k, positions, inv_freq, layout, scale):
     return _rope_state(q)[1], _rope_state(k)[1]
 
 
-rope_positions.register_fake(_rope_positions_fake)
-rope_positions_backward.register_fake(_rope_positions_fake)
+class _RopePositions(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, layout, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.layout, ctx.scale = layout, scale
+        ctx.metas = [(t.shape, t.dtype, t.device) for t in (q, k)]
+        ctx.set_materialize_grads(False)
+        return _below_autograd(rope_positions, q, k, positions, inv_freq, layout, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        grads = [torch.zeros(shape, dtype=dtype, device=device) if g is None else g
+                 for g, (shape, dtype, device) in zip(grads, ctx.metas)]
+        return (*rope_positions_backward(*grads, *ctx.saved_tensors, ctx.layout, ctx.scale),
+                None, None, None, None)
 
 
-def _rope_positions_setup(ctx, inputs, output) -> None:
-    q, k, positions, inv_freq, ctx.layout, ctx.scale = inputs
-    ctx.save_for_backward(positions, inv_freq)
-    ctx.q_meta = (q.shape, q.dtype, q.device)
-    ctx.k_meta = (k.shape, k.dtype, k.device)
-    ctx.set_materialize_grads(False)
-
-
-def _rope_positions_bwd(ctx, dq: Tensor | None, dk: Tensor | None):
-    positions, inv_freq = ctx.saved_tensors
-    if dq is None:
-        dq = torch.zeros(ctx.q_meta[0], dtype=ctx.q_meta[1], device=ctx.q_meta[2])
-    if dk is None:
-        dk = torch.zeros(ctx.k_meta[0], dtype=ctx.k_meta[1], device=ctx.k_meta[2])
-    gq, gk = torch.ops.picotron_b200.rope_positions_backward(dq, dk, positions, inv_freq,
-                                                             ctx.layout, ctx.scale)
-    return gq, gk, None, None, None, None
-
-
-rope_positions.register_autograd(_rope_positions_bwd, setup_context=_rope_positions_setup)
+_ROPE_POSITIONS = ("(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, int layout, "
+                   "float scale) -> (Tensor, Tensor)")
+rope_positions_backward = _register("rope_positions_backward" + _ROPE_POSITIONS,
+                                    _rope_positions_backward, _rope_positions_fake)
+rope_positions = _register("rope_positions" + _ROPE_POSITIONS, _rope_positions,
+                           _rope_positions_fake, _RopePositions)

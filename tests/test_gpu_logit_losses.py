@@ -23,6 +23,7 @@ import torch
 import gpu_utils as gu
 from picotron_b200 import _capi, kernels
 from picotron_b200.errors import TritonLogitLossUnavailable
+from picotron_b200.ops import DTYPE_CODES
 
 pytestmark = pytest.mark.gpu
 
@@ -388,6 +389,85 @@ def test_policy_advantage_per_sequence_equals_broadcast():
     assert torch.equal(a, b) and torch.equal(da, db)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("expected", [None, 1.0, 0.25, 3.0, -2.0])
+def test_policy_expected_gradient(dtype, expected):
+    """The gradient is right whatever the loss's gradient turns out to be; formed for another
+    factor it is rounded twice."""
+
+    x, t = _data((3, 7, 1003), dtype, seed=33)
+    old, ref, adv = _policy_inputs(x, t, 34)
+    _, coef, bend, _ = _policy64(_logps64(x, t), old, adv, ref, t, 0.2, 0.2, 0.1, False)
+    eps, info = _eps(1003), torch.finfo(dtype)
+    for up in (1.0, 0.25, 3.0):
+        leaf = x.detach().requires_grad_()
+        loss, _ = kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref, kl_coef=0.1,
+                                      expected_grad=expected)
+        grads = [torch.autograd.grad(loss, leaf, torch.tensor(up, device=gu.DEV),
+                                     retain_graph=True)[0] for _ in range(3)]
+        assert torch.equal(grads[1], grads[2])  # the second and third are formed in backward
+        # Formed once at full precision.
+        _check_grad(grads[1], x, t, up * coef, up * (1.01 * eps * bend + 2 * U * coef.abs()))
+        want, p = _grad64(x, t, up * coef)
+        formed = expected or 1.0
+        extra = 0.0 if up == expected else (
+            info.eps / 2 * want.abs() + abs(up / formed) * info.smallest_normal * info.eps)
+        tol = (up * coef.abs().unsqueeze(-1) * p * 2 * eps
+               + up * (1.01 * eps * bend + 2 * U * coef.abs()).unsqueeze(-1)
+               + want.abs() * (8 * U + info.eps / 2) + info.smallest_normal * info.eps + extra)
+        assert ((grads[0].double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("vocab,dtype", [(400_001, torch.float32), (786_440, torch.bfloat16)],
+                         ids=str)
+def test_policy_rows_that_do_not_fit_on_chip(vocab, dtype):
+    x, t = _data((1, 3, vocab), dtype, seed=35, ignore=False)
+    old, ref, adv = _policy_inputs(x, t, 36)
+    assert not _capi.policy_loss_grad_supported(vocab, 1, 3, DTYPE_CODES[dtype])
+    _check_policy(x, t, old, adv, ref, 0.1, "token", scales=(None,))
+
+
+@pytest.mark.parametrize("vocab,dtype", [(393_216, torch.float32), (262_145, torch.float32),
+                                         (262_144, torch.bfloat16), (262_151, torch.bfloat16)],
+                         ids=str)
+def test_policy_rows_that_just_fit_on_chip(vocab, dtype):
+    x, t = _data((1, 3, vocab), dtype, seed=37, ignore=False)
+    old, ref, adv = _policy_inputs(x, t, 38)
+    _check_policy(x, t, old, adv, ref, 0.1, "token", scales=(None,))
+
+
+@pytest.mark.parametrize("view", VIEWS)
+def test_policy_of_views(view):
+    for dtype, vocab in ((torch.bfloat16, 1001), (torch.float32, 64)):
+        x, t = _data((4, 6, vocab), dtype, seed=39)
+        x, t = VIEWS[view](x, t)
+        if t.numel() == 0:
+            continue
+        old, ref, adv = _policy_inputs(x, t, 40)
+        _check_policy(x, t, old, adv, ref, 0.1, "token", scales=(None,))
+
+
+def test_compiled_graphs_agree():
+    x, t = _data((2, 6, 501), torch.bfloat16, seed=47)
+    old, ref, adv = _policy_inputs(x, t, 48)
+
+    def run(leaf):
+        lp = kernels.token_log_probs(leaf, t)
+        pref, _ = kernels.preference_loss(leaf, t, ref)
+        pol, _ = kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref, kl_coef=0.1)
+        return lp.sum() + pref + pol
+
+    grads = []
+    for f in (run, torch.compile(run, backend="aot_eager", fullgraph=True)):
+        leaf = x.detach().requires_grad_()
+        loss = f(leaf)
+        loss.backward()
+        grads.append((loss.detach(), leaf.grad))
+    assert torch.equal(grads[0][0], grads[1][0])
+    # Three gradients added in bf16, each rounded: half a step of the largest partial sums.
+    assert (grads[0][1] - grads[1][1]).abs().max() <= 2 ** -7 * grads[0][1].abs().max()
+
+
 def test_policy_2d_and_unclipped():
     x, t = _data((1, 50, 777), torch.float32, seed=27)
     old, ref, adv = _policy_inputs(x, t, 28, 0.9, 2.0)
@@ -524,6 +604,8 @@ def test_refusals():
         lambda: kernels.policy_loss(x, t, f, f, clip_low=-0.1),
         lambda: kernels.policy_loss(x, t, f, f, clip_high=math.nan),
         lambda: kernels.policy_loss(x, t, f, f, aggregate="sum"),
+        lambda: kernels.policy_loss(x, t, f, f, expected_grad=0.0),
+        lambda: kernels.policy_loss(x, t, f, f, expected_grad=math.nan),
         lambda: kernels.policy_loss(x, t, f.cpu(), f),
     ]
     for call in bad:

@@ -68,6 +68,22 @@ def test_loss_entry_points_reject_bad_arguments_before_cuda():
     assert "kl_coef" in _capi.last_error()
 
 
+def test_policy_gradient_support_and_rescaling_are_checked_before_cuda():
+    lib, flag = _capi.library(), ctypes.c_int(-1)
+    ask = lambda vocab, outer=1, dtype=2: (  # noqa: E731
+        lib.pt_policy_loss_grad_supported(vocab, outer, 1, dtype, ctypes.byref(flag)), flag.value)
+    assert ask(128256) == (_capi.PT_OK, 1) and ask(786432) == (_capi.PT_OK, 1)
+    assert ask(786433) == (_capi.PT_OK, 0) and ask(400_000, dtype=0) == (_capi.PT_OK, 0)
+    assert ask(8, 2**29) == (_capi.PT_OK, 0)
+    assert ask(0)[0] == _capi.PT_ERR_SHAPE and ask(8, dtype=4)[0] == _capi.PT_ERR_UNSUPPORTED_DTYPE
+    rescale = lambda expected, dtype=2, outer=1: lib.pt_rescale_logits_grad(  # noqa: E731
+        None, 8, outer, 1, 8, 8, None, expected, dtype, None)
+    assert rescale(0.0) == rescale(math.nan) == _capi.PT_ERR_INVALID_ARGUMENT
+    assert rescale(1.0, dtype=3) == _capi.PT_ERR_UNSUPPORTED_DTYPE
+    assert rescale(1.0, outer=-1) == _capi.PT_ERR_SHAPE
+    assert rescale(1.0, outer=0) == _capi.PT_OK
+
+
 def test_adamw8_entry_points_reject_bad_arguments_before_cuda():
     lib = _capi.library()
     one = (ctypes.c_void_p * 1)(None)
@@ -175,7 +191,8 @@ def test_fake_implementations_match_shapes_and_strides():
         assert lp.shape == (2, 3) and lp.dtype == torch.float32 and stats.shape == (2, 3, 2)
         out = torch.ops.picotron_b200.preference_loss(x, t, f, 0.1, 0.0, -100)
         assert [tuple(o.shape) for o in out] == [(), (2,), (2, 3, 2), (2,)]
-        out = torch.ops.picotron_b200.policy_loss(x, t, f, f, None, 0.2, 0.2, 0.0, False, -100)
+        out = torch.ops.picotron_b200.policy_loss(x, t, f, f, None, 0.2, 0.2, 0.0, False, -100,
+                                                  None)
         assert [tuple(o.shape) for o in out] == [(), (2, 3), (2, 3, 2), (2, 3)]
         back = torch.ops.picotron_b200.logit_loss_backward
         assert back(x, t, stats, f, None, -100).stride() == x.stride()
