@@ -384,7 +384,8 @@ PT_API int pt_cross_entropy_bwd(const void* logits, int64_t vocab, int64_t outer
 
 /* The logit losses read rows of `vocab` logits as pt_cross_entropy_fwd does: an [outer, inner]
  * grid (sequences x positions) with two row strides in elements, class stride 1, an int64
- * target per row with its own two strides, f32 / f16 / bf16 logits, fp32 math. Rows whose
+ * target per row with its own two strides, f32 / f16 / bf16 logits, fp32 math, fewer than 2^31
+ * rows. Rows whose
  * target is ignore_index are not read: they have no log-probability (0 is written), no part in
  * any loss and a gradient of zeros, whatever their logits and per-token inputs hold. A target
  * outside [0, vocab) gives NaN and sets the device error word; its gradient is zeros. A row

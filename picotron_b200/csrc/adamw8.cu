@@ -10,31 +10,38 @@
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g g       (every product and sum rounded)
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Each new code is the one nearest to the new fp32 moment in the root's domain. The candidate
-// comes from the approximate square root; where it lies within 2e-4 of a border between two
-// codes (above the 6e-5 that the approximations can be off by at code 255), the border itself,
+// comes from the approximate square root; where it lies within 1e-4 of a border between two
+// codes (above the 5.7e-5 that reciprocal, product and two square roots, 2^-23 each, can be off
+// by at code 255), the border itself,
 // ((2c + 1) / 2)^2 s or ((2c + 1) / 2)^4 s, is compared with the moment in 64 bits, so the code
 // does not depend on how the root was computed.
 //
-// One warp per block of 256: eight elements per lane in 32-byte loads, the block's two maxima by
-// integer max over the warp (for values >= 0 the bit patterns order like the values, NaN above
-// all). Bytes per element: 3 parameter widths (parameter read and written, gradient read) + 4;
+// One warp per block of 256, eight elements per lane; the block's two maxima by integer max over
+// the warp (for values >= 0 the bit patterns order like the values, NaN above all). Bytes per element: 3 parameter widths (parameter read and written, gradient read) + 4;
 // the kernel is bound by HBM.
+#include <algorithm>
 #include <cmath>
 
 #include "common.cuh"
 
 namespace pt {
+
+__device__ int g_adamw8_error = 0;
+
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;            // elements that share a scale
-constexpr int kWarpBlocks = 4;         // quantisation blocks per warp and work item
-constexpr int kItemBlocks = kThreads / 32 * kWarpBlocks;  // per work item (8192 elements)
+
+constexpr int kWarps = kThreads / 32;
+constexpr int kStages = 2;             // blocks that a warp's copies run ahead (see adamw8_kernel)
+constexpr int kMaxWarpBlocks = 16;     // blocks per warp and work item, at most
 constexpr int kBatch = 96;             // tensors per launch (10 KB of kernel parameters)
 constexpr float kTiny = 1.17549435e-38f;  // smallest normal: a smaller scale is kept as 0
 constexpr float kMomentScale = (float)(1.0 / 16129.0);        // 127^-2
 constexpr float kSquareScale = (float)(1.0 / 4228250625.0);   // 255^-4
-constexpr float kBorder = 0.4998f;
+constexpr float kBorder = 0.4999f;
+
 
 struct Tensor {
   void* param;
@@ -53,6 +60,7 @@ struct Tensor {
 struct Batch {
   Tensor t[kBatch];
   int count;
+  int warp_blocks;  // blocks per warp and work item
 };
 
 struct Scalars {
@@ -62,171 +70,348 @@ struct Scalars {
 
 __device__ __forceinline__ float approx_sqrt(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float approx_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The larger of two values >= 0, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float warp_top(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
 
-// The eight codes of one lane's part of a block.
-struct Codes {
-  int8_t m[8];
-  uint8_t v[8];
+// The sum of two pairs of products, each product rounded and then the sum. Packed products and
+// sums (mul and add of f32x2, .rn in PTX as well) were contracted into fused multiply-adds, which
+// the definition of the moments rules out; scalar sums with explicit rounding are not.
+__device__ __forceinline__ float2 sum_of_products(float2 a, float2 wa, float2 b, float2 wb) {
+  const float2 x = __fmul2_rn(a, wa), y = __fmul2_rn(b, wb);
+  return make_float2(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+}
+
+// Whole numbers in the low byte of an fp32: x + kWhole is x rounded to the nearest whole number,
+// ties to even, whose two's complement is the low bits (|x| < 2^22).
+constexpr float kWhole = 12582912.0f;  // 1.5 * 2^23
+
+// Byte e of w as an fp32: 2^23 with the byte in its low bits, less 2^23 and `bias`.
+__device__ __forceinline__ float2 bytes_to_float2(uint32_t w, int e, float bias) {
+  const uint32_t a = __byte_perm(w, 0x4b000000u, 0x7440 + e);
+  const uint32_t b = __byte_perm(w, 0x4b000000u, 0x7441 + e);
+  return __fadd2_rn(make_float2(__uint_as_float(a), __uint_as_float(b)), splat2(-8388608.0f - bias));
+}
+// The low bytes of four values that kWhole was added to.
+__device__ __forceinline__ uint32_t low_bytes(float2 a, float2 b) {
+  const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
+// Eight moments of one lane as codes, and the values that codes stand for. Every product that is
+// part of the definition is rounded by itself.
+__device__ __forceinline__ void moment_values(uint2 codes, float scale, float2 (&m)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // int8 as a byte with 128 added.
+    float2 c = bytes_to_float2((i < 2 ? codes.x : codes.y) ^ 0x80808080u, 2 * (i & 1), 128.0f);
+    c = make_float2(c.x * fabsf(c.x), c.y * fabsf(c.y));
+    m[i] = __fmul2_rn(c, splat2(scale));
+  }
+}
+__device__ __forceinline__ void square_values(uint2 codes, float scale, float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 c = bytes_to_float2(i < 2 ? codes.x : codes.y, 2 * (i & 1), 0.0f);
+    c = __fmul2_rn(c, c);
+    v[i] = __fmul2_rn(__fmul2_rn(c, c), splat2(scale));
+  }
+}
+
+// The exact choice between codes lo and lo + 1 for a root next to lo + 1/2: the moment (times
+// 2^power) against the border (2 lo + 1)^power s, both exact or within 2^-53; ties to even.
+template <int kPower>
+__device__ __noinline__ float border_code(float root, float x, float s) {
+  const int lo = (int)floorf(root);
+  double b = (double)(2 * lo + 1);
+  b *= b;
+  if (kPower == 4) b *= b;
+  const double border = b * (double)s, value = (double)(1 << kPower) * (double)x;
+  return (float)(value > border || (value == border && (lo & 1)) ? lo + 1 : lo);
+}
+
+// How far a root is from the whole number that it was rounded to in `t`.
+__device__ __forceinline__ float off_whole(float root, float t) {
+  return fabsf(__fsub_rn(root, __fsub_rn(t, kWhole)));
+}
+__device__ __forceinline__ float2 to_whole(float2 root, float& worst) {
+  const float2 t = __fadd2_rn(root, splat2(kWhole));
+  const float2 c = __fadd2_rn(t, splat2(-kWhole));
+  const float2 d = __fadd2_rn(root, make_float2(-c.x, -c.y));
+  worst = fmaxf(worst, fmaxf(fabsf(d.x), fabsf(d.y)));
+  return t;
+}
+
+// The codes nearest to eight moments in the root's domain; zeros, which stand for NaN, under a
+// scale that is not finite.
+__device__ __forceinline__ uint2 moment_codes(const float2 (&m)[4], float s) {
+  if (!(s < INFINITY)) return make_uint2(0, 0);
+  const float inv = s > 0.0f ? approx_rcp(s) : 0.0f;
+  float2 r[4], t[4];
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 q = __fmul2_rn(m[i], splat2(inv));
+    r[i] = make_float2(copysignf(approx_sqrt(fabsf(q.x)), m[i].x),
+                       copysignf(approx_sqrt(fabsf(q.y)), m[i].y));
+    t[i] = to_whole(r[i], worst);
+  }
+  if (worst > kBorder) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (off_whole(r[i].x, t[i].x) > kBorder)
+        t[i].x = kWhole + copysignf(border_code<2>(fabsf(r[i].x), fabsf(m[i].x), s), m[i].x);
+      if (off_whole(r[i].y, t[i].y) > kBorder)
+        t[i].y = kWhole + copysignf(border_code<2>(fabsf(r[i].y), fabsf(m[i].y), s), m[i].y);
+    }
+  }
+  return make_uint2(low_bytes(t[0], t[1]), low_bytes(t[2], t[3]));
+}
+__device__ __forceinline__ uint2 square_codes(const float2 (&v)[4], float s) {
+  if (!(s < INFINITY)) return make_uint2(0, 0);
+  const float inv = s > 0.0f ? approx_rcp(s) : 0.0f, least = s > 0.0f ? 1.0f : 0.0f;
+  float2 r[4], t[4];
+  float worst = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 q = __fmul2_rn(v[i], splat2(inv));
+    r[i] = make_float2(approx_sqrt(approx_sqrt(q.x)), approx_sqrt(approx_sqrt(q.y)));
+    if (v[i].x > 0.0f) r[i].x = fmaxf(r[i].x, least);
+    if (v[i].y > 0.0f) r[i].y = fmaxf(r[i].y, least);
+    t[i] = to_whole(r[i], worst);
+  }
+  if (worst > kBorder) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (off_whole(r[i].x, t[i].x) > kBorder) t[i].x = kWhole + border_code<4>(r[i].x, v[i].x, s);
+      if (off_whole(r[i].y, t[i].y) > kBorder) t[i].y = kWhole + border_code<4>(r[i].y, v[i].y, s);
+    }
+  }
+  return make_uint2(low_bytes(t[0], t[1]), low_bytes(t[2], t[3]));
+}
+
+struct StepScalars {
+  float step_size, root, decay;
 };
 
-// sqrt(q) rounded to the nearest code, ties to even; x = |moment|, q = x / s approximately.
-__device__ __forceinline__ int moment_code(float x, float s, float inv) {
-  const float r = approx_sqrt(x * inv);
-  float c = rintf(r);
-  if (fabsf(r - c) > kBorder) {
-    const int lo = (int)floorf(r);
-    const double b = (double)(2 * lo + 1);
-    const double border = b * b * (double)s, value = 4.0 * (double)x;
-    c = (float)(value > border || (value == border && (lo & 1)) ? lo + 1 : lo);
-  }
-  return min((int)c, 127);
-}
-
-__device__ __forceinline__ int square_code(float x, float s, float inv) {
-  const float r = approx_sqrt(approx_sqrt(x * inv));
-  float c = rintf(r);
-  if (fabsf(r - c) > kBorder) {
-    const int lo = (int)floorf(r);
-    double b = (double)(2 * lo + 1);
-    b *= b;
-    const double border = b * b * (double)s, value = 16.0 * (double)x;
-    c = (float)(value > border || (value == border && (lo & 1)) ? lo + 1 : lo);
-  }
-  const int code = min((int)c, 255);
-  return code == 0 && x > 0.0f && s > 0.0f ? 1 : code;
-}
-
-__device__ __forceinline__ float moment_value(int c, float s) { return (float)(c * abs(c)) * s; }
-__device__ __forceinline__ float square_value(int c, float s) {
-  const float d = (float)(c * c);
-  return __fmul_rn(__fmul_rn(d, d), s);
-}
-
-// The step of one warp's block: p, g and the codes of this lane in registers (elements past the
-// end hold g = 0 and codes 0, so they change no maximum). ms, vs: the block's scales, in and out.
-__device__ __forceinline__ void step_block(float (&p)[8], const float (&g)[8], Codes& q, float& ms,
-                                           float& vs, const Scalars& k, const Tensor& t) {
-  float m[8], v[8];
-  uint32_t mtop = 0, vtop = 0;
+// The parameters' step on one warp's block, and its new moments: p, g and the codes of this lane
+// in registers (elements past the end hold g = 0 and codes 0, so they change no maximum). ms, vs:
+// the block's scales, in and out.
+__device__ __forceinline__ void step_block(float2 (&p)[4], const float2 (&g)[4], uint2 mc,
+                                           uint2 vc, float2 (&m)[4], float2 (&v)[4], float& ms,
+                                           float& vs, const Scalars& k, const StepScalars& t) {
+  moment_values(mc, ms, m);
+  square_values(vc, vs, v);
+  float mtop = 0.0f, vtop = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float ge = k.maximize ? -g[e] : g[e];
-    m[e] = __fadd_rn(__fmul_rn(moment_value(q.m[e], ms), k.b1), __fmul_rn(ge, k.w1));
-    v[e] = __fadd_rn(__fmul_rn(square_value(q.v[e], vs), k.b2),
-                     __fmul_rn(__fmul_rn(ge, ge), k.w2));
-    mtop = max(mtop, __float_as_uint(fabsf(m[e])));
-    vtop = max(vtop, __float_as_uint(v[e]));
-    const float d = fmaf(approx_sqrt(v[e]), t.root, k.eps);
-    p[e] = fmaf(-t.step_size, __fdividef(m[e], d), p[e] * t.decay);
+  for (int i = 0; i < 4; ++i) {
+    m[i] = sum_of_products(m[i], splat2(k.b1), g[i], splat2(k.w1));
+    v[i] = sum_of_products(v[i], splat2(k.b2), __fmul2_rn(g[i], g[i]), splat2(k.w2));
+    mtop = max_nan(mtop, max_nan(fabsf(m[i].x), fabsf(m[i].y)));
+    vtop = max_nan(vtop, max_nan(v[i].x, v[i].y));
+    const float2 d = __ffma2_rn(make_float2(approx_sqrt(v[i].x), approx_sqrt(v[i].y)),
+                                splat2(t.root), splat2(k.eps));
+    const float2 u = __fmul2_rn(m[i], make_float2(approx_rcp(d.x), approx_rcp(d.y)));
+    p[i] = __ffma2_rn(u, splat2(-t.step_size), __fmul2_rn(p[i], splat2(t.decay)));
   }
-  ms = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, mtop)), kMomentScale);
-  vs = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, vtop)), kSquareScale);
+  ms = __fmul_rn(warp_top(mtop), kMomentScale);
+  vs = __fmul_rn(warp_top(vtop), kSquareScale);
   ms = ms < kTiny ? 0.0f : ms;
   vs = vs < kTiny ? 0.0f : vs;
-  const float mi = ms > 0.0f ? __fdividef(1.0f, ms) : 0.0f;
-  const float vi = vs > 0.0f ? __fdividef(1.0f, vs) : 0.0f;
+}
+
+// Eight elements from shared memory.
+template <typename T> __device__ __forceinline__ void lds8(const T* p, float2 (&f)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    unpack2<T>(lds128(p), f);
+    unpack2<T>(lds128(p + 4), f + 2);
+  } else {
+    unpack2<T>(lds128(p), f);
+  }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float2 (&f)[4]) {
+  float t[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = moment_code(fabsf(m[e]), ms, mi);
-    q.m[e] = (int8_t)(m[e] < 0.0f ? -c : c);
-    q.v[e] = (uint8_t)square_code(v[e], vs, vi);
+  for (int i = 0; i < 4; ++i) {
+    t[2 * i] = f[i].x;
+    t[2 * i + 1] = f[i].y;
   }
+  if constexpr (sizeof(T) == 4)
+    st_global_v8(p, t);
+  else
+    *reinterpret_cast<uint4*>(p) = pack<T>(t);
 }
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    ld_global_v8(p, f);
-  } else {
-    unpack<T>(*reinterpret_cast<const uint4*>(p), f);
+// The tensor that a work item belongs to (items of tensor i end at t[i].item_end).
+template <typename B> __device__ __forceinline__ int tensor_of(const B& batch, int64_t item) {
+  int lo = 0, hi = batch.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (item < batch.t[mid].item_end)
+      hi = mid;
+    else
+      lo = mid + 1;
   }
-}
-template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    st_global_v8(p, f);
-  } else {
-    *reinterpret_cast<uint4*>(p) = pack<T>(f);
-  }
+  return lo;
 }
 
+// What one warp's block takes from memory, as it lies in shared memory: 256 elements of each.
+template <typename T> struct Stage {
+  T p[kBlock];
+  T g[kBlock];
+  int8_t mc[kBlock];
+  uint8_t vc[kBlock];
+};
+
+// A warp's whole blocks come through a ring of kStages stages in shared memory, filled by bulk
+// copies that run ahead: with plain loads the time followed the number of resident warps (2.8,
+// 2.1 and 1.7 ms with 2, 3 and 4 CTAs per SM), since a block's loads waited for the arithmetic of
+// the one before. 436 M fp32 parameters take 1.07 ms, the time of their bytes at the copy rate,
+// with 16 blocks a warp, 2 stages and 3 CTAs per SM (1.08 ms with 8 blocks, 1.25 with 4; 1.09
+// with 3 stages; 1.09 with 4 CTAs, 1.10 with 2 CTAs of 3 stages).
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 adamw8_kernel(const __grid_constant__ Batch batch, Scalars k) {
+  extern __shared__ __align__(128) unsigned char shared[];
+  __shared__ uint64_t bars[kWarps][kStages];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t items = batch.t[batch.count - 1].item_end;
-  int i = 0;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    while (item >= batch.t[i].item_end) ++i;  // items are visited in increasing order
-    const Tensor& t = batch.t[i];
-    const int64_t first = i > 0 ? batch.t[i - 1].item_end : 0;
-    T* P = static_cast<T*>(t.param);
-    const T* G = static_cast<const T*>(t.grad);
-    const uintptr_t wide = reinterpret_cast<uintptr_t>(P) | reinterpret_cast<uintptr_t>(G);
-    const uintptr_t codes = reinterpret_cast<uintptr_t>(t.mc) | reinterpret_cast<uintptr_t>(t.vc);
-    const bool aligned = wide % (8 * sizeof(T)) == 0 && codes % 8 == 0;
-    const int64_t blocks = (t.numel + kBlock - 1) / kBlock;
-    const int64_t b0 = (item - first) * kItemBlocks + warp;
-    for (int j = 0; j < kWarpBlocks; ++j) {
-      const int64_t b = b0 + j * (kThreads / 32);
-      if (b >= blocks) break;
-      float ms = t.ms[b], vs = t.vs[b];
-      float p[8], g[8];
-      Codes q;
-      const int64_t at = b * kBlock;
-      if (aligned && at + kBlock <= t.numel) {
-        const int64_t o = at + lane * 8;
-        load8<T>(P + o, p);
-        load8<T>(G + o, g);
-        const uint2 mc = *reinterpret_cast<const uint2*>(t.mc + o);
-        const uint2 vc = *reinterpret_cast<const uint2*>(t.vc + o);
+  const int64_t item = blockIdx.x;
+  const int which = tensor_of(batch, item);
+  const Tensor& t = batch.t[which];
+  const int64_t first = which > 0 ? batch.t[which - 1].item_end : 0;
+  T* const P = static_cast<T*>(t.param);
+  const T* const G = static_cast<const T*>(t.grad);
+  int8_t* const MC = t.mc;
+  uint8_t* const VC = t.vc;
+  const int64_t numel = t.numel;
+  const StepScalars sc{t.step_size, t.root, t.decay};
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(P) | reinterpret_cast<uintptr_t>(G) |
+                         reinterpret_cast<uintptr_t>(MC) | reinterpret_cast<uintptr_t>(VC);
+  // Whole blocks of arrays on 32-byte boundaries; anything else goes element by element.
+  const int64_t whole = bits % 32 == 0 ? numel / kBlock : 0;
+  const int64_t blocks = (numel + kBlock - 1) / kBlock;
+  const int64_t b0 = ((item - first) * kWarps + warp) * batch.warp_blocks;  // consecutive blocks
+  const int n = (int)max((int64_t)0, min((int64_t)batch.warp_blocks, whole - b0));
+  Stage<T>* ring = reinterpret_cast<Stage<T>*>(shared) + warp * kStages;
+  uint64_t* bar = bars[warp];
+  auto fetch = [&](int j) {  // by lane 0
+    Stage<T>& s = ring[j % kStages];
+    uint64_t* at = &bar[j % kStages];
+    const int64_t o = (b0 + j) * kBlock;
+    mbar_arrive_expect_tx(at, sizeof(Stage<T>));
+    bulk_load(s.p, P + o, sizeof(s.p), at);
+    bulk_load(s.g, G + o, sizeof(s.g), at);
+    bulk_load(s.mc, MC + o, sizeof(s.mc), at);
+    bulk_load(s.vc, VC + o, sizeof(s.vc), at);
+  };
+  if (lane == 0 && n > 0) {
+    for (int j = 0; j < kStages; ++j) mbar_init(&bar[j], 1);
+    fence_mbar_init();
+    for (int j = 0; j < min(n, kStages); ++j) fetch(j);
+  }
+  __syncwarp();
+  float ms = 0.0f, vs = 0.0f;
+  if (n > 0) {
+    ms = t.ms[b0];
+    vs = t.vs[b0];
+  }
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    const int64_t b = b0 + j;
+    float next_ms = 0.0f, next_vs = 0.0f;
+    if (j + 1 < n) {
+      next_ms = t.ms[b + 1];
+      next_vs = t.vs[b + 1];
+    }
+    if (!mbar_wait_bounded(&bar[j % kStages], (uint32_t)(j / kStages) & 1u)) {
+      // Nothing of this block, or of the warp's blocks behind it, is changed; the copies that are
+      // still on their way are given their time as well.
+      if (lane == 0) atomicExch(&g_adamw8_error, kDeviceErrWaitTimeout);
+      for (int i = j + 1; i < min(n, j + kStages); ++i)
+        mbar_wait_bounded(&bar[i % kStages], (uint32_t)(i / kStages) & 1u);
+      return;
+    }
+    const Stage<T>& s = ring[j % kStages];
+    float2 p[4], g[4], m[4], v[4];
+    lds8<T>(s.p + lane * 8, p);
+    lds8<T>(s.g + lane * 8, g);
+    const uint2 mc = *reinterpret_cast<const uint2*>(s.mc + lane * 8);
+    const uint2 vc = *reinterpret_cast<const uint2*>(s.vc + lane * 8);
+    __syncwarp();  // all lanes have read the stage
+    if (lane == 0 && j + kStages < n) fetch(j + kStages);
+    if (k.maximize)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          q.m[e] = (int8_t)((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
-          q.v[e] = (uint8_t)((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)));
-        }
-        step_block(p, g, q, ms, vs, k, t);
-        store8<T>(P + o, p);
-        uint2 mo = make_uint2(0, 0), vo = make_uint2(0, 0);
+      for (int i = 0; i < 4; ++i) g[i] = make_float2(-g[i].x, -g[i].y);
+    step_block(p, g, mc, vc, m, v, ms, vs, k, sc);
+    const int64_t o = b * kBlock + lane * 8;
+    store8<T>(P + o, p);
+    *reinterpret_cast<uint2*>(MC + o) = moment_codes(m, ms);
+    *reinterpret_cast<uint2*>(VC + o) = square_codes(v, vs);
+    if (lane == 0) {
+      t.ms[b] = ms;
+      t.vs[b] = vs;
+    }
+    ms = next_ms;
+    vs = next_vs;
+  }
+#pragma unroll 1
+  for (int64_t b = max(b0, whole); b < min(b0 + batch.warp_blocks, blocks); ++b) {
+    float2 p[4], g[4], m[4], v[4];
+    float pe[8], ge[8];
+    uint2 mc = make_uint2(0, 0), vc = make_uint2(0, 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          (e < 4 ? mo.x : mo.y) |= (uint32_t)(uint8_t)q.m[e] << (8 * (e & 3));
-          (e < 4 ? vo.x : vo.y) |= (uint32_t)q.v[e] << (8 * (e & 3));
-        }
-        *reinterpret_cast<uint2*>(t.mc + o) = mo;
-        *reinterpret_cast<uint2*>(t.vc + o) = vo;
-      } else {
-        // A short last block, or arrays that are not aligned: lane strides of one element.
+    for (int e = 0; e < 8; ++e) {
+      const int64_t o = b * kBlock + e * 32 + lane;
+      const bool in = o < numel;
+      pe[e] = in ? to_float(P[o]) : 0.0f;
+      ge[e] = in ? to_float(G[o]) : 0.0f;
+      ge[e] = k.maximize ? -ge[e] : ge[e];
+      (e < 4 ? mc.x : mc.y) |= (in ? (uint32_t)(uint8_t)MC[o] : 0u) << (8 * (e & 3));
+      (e < 4 ? vc.x : vc.y) |= (in ? (uint32_t)VC[o] : 0u) << (8 * (e & 3));
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int64_t o = at + e * 32 + lane;
-          const bool in = o < t.numel;
-          p[e] = in ? to_float(P[o]) : 0.0f;
-          g[e] = in ? to_float(G[o]) : 0.0f;
-          q.m[e] = in ? t.mc[o] : (int8_t)0;
-          q.v[e] = in ? t.vc[o] : (uint8_t)0;
-        }
-        step_block(p, g, q, ms, vs, k, t);
+    for (int i = 0; i < 4; ++i) {
+      p[i] = make_float2(pe[2 * i], pe[2 * i + 1]);
+      g[i] = make_float2(ge[2 * i], ge[2 * i + 1]);
+    }
+    float bms = t.ms[b], bvs = t.vs[b];
+    step_block(p, g, mc, vc, m, v, bms, bvs, k, sc);
+    mc = moment_codes(m, bms);
+    vc = square_codes(v, bvs);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int64_t o = at + e * 32 + lane;
-          if (o < t.numel) {
-            P[o] = from_float<T>(p[e]);
-            t.mc[o] = q.m[e];
-            t.vc[o] = q.v[e];
-          }
-        }
+    for (int e = 0; e < 8; ++e) {
+      const int64_t o = b * kBlock + e * 32 + lane;
+      if (o < numel) {
+        P[o] = from_float<T>(e & 1 ? p[e / 2].y : p[e / 2].x);
+        MC[o] = (int8_t)((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
+        VC[o] = (uint8_t)((e < 4 ? vc.x : vc.y) >> (8 * (e & 3)));
       }
-      if (lane == 0) {
-        t.ms[b] = ms;
-        t.vs[b] = vs;
-      }
+    }
+    if (lane == 0) {
+      t.ms[b] = bms;
+      t.vs[b] = bvs;
     }
   }
 }
 
-// The fp32 moments that codes and scales stand for.
+// The fp32 moments that codes and scales stand for: 10 bytes per element, most of them written.
+// 436 M elements take 0.65 ms, the copy rate (0.68 ms with 8 or 16 blocks a warp).
+constexpr int kMomentWarpBlocks = 4;
 struct MomentTensor {
   const int8_t* mc;
   const float* ms;
@@ -240,58 +425,63 @@ struct MomentTensor {
 struct MomentBatch {
   MomentTensor t[kBatch];
   int count;
+  int warp_blocks;
 };
 
 __global__ void __launch_bounds__(kThreads)
 moments_kernel(const __grid_constant__ MomentBatch batch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t items = batch.t[batch.count - 1].item_end;
-  int i = 0;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    while (item >= batch.t[i].item_end) ++i;
-    const MomentTensor& t = batch.t[i];
-    const int64_t first = i > 0 ? batch.t[i - 1].item_end : 0;
-    const bool aligned =
-        (reinterpret_cast<uintptr_t>(t.mc) | reinterpret_cast<uintptr_t>(t.vc)) % 8 == 0 &&
-        (reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) % 32 == 0;
-    const int64_t blocks = (t.numel + kBlock - 1) / kBlock;
-    const int64_t b0 = (item - first) * kItemBlocks + warp;
-#pragma unroll
-    for (int j = 0; j < kWarpBlocks; ++j) {
-      const int64_t b = b0 + j * (kThreads / 32);
-      if (b >= blocks) break;
-      const float ms = t.ms[b], vs = t.vs[b];
-      const int64_t at = b * kBlock;
-      if (aligned && at + kBlock <= t.numel) {
-        const int64_t o = at + lane * 8;
-        const uint2 mc = *reinterpret_cast<const uint2*>(t.mc + o);
-        const uint2 vc = *reinterpret_cast<const uint2*>(t.vc + o);
-        float m[8], v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          m[e] = moment_value((int8_t)((e < 4 ? mc.x : mc.y) >> (8 * (e & 3))), ms);
-          v[e] = square_value((uint8_t)((e < 4 ? vc.x : vc.y) >> (8 * (e & 3))), vs);
-        }
-        st_global_v8(t.m + o, m);
-        st_global_v8(t.v + o, v);
-      } else {
-        for (int64_t o = at + lane; o < min(at + kBlock, t.numel); o += 32) {
-          t.m[o] = moment_value(t.mc[o], ms);
-          t.v[o] = square_value(t.vc[o], vs);
-        }
+  const int64_t item = blockIdx.x;
+  const int which = tensor_of(batch, item);
+  const MomentTensor t = batch.t[which];
+  const int64_t first = which > 0 ? batch.t[which - 1].item_end : 0;
+  const bool aligned =
+      (reinterpret_cast<uintptr_t>(t.mc) | reinterpret_cast<uintptr_t>(t.vc)) % 8 == 0 &&
+      (reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) % 32 == 0;
+  const int64_t blocks = (t.numel + kBlock - 1) / kBlock;
+  const int64_t b0 = (item - first) * batch.warp_blocks * kWarps + warp;
+#pragma unroll 4
+  for (int j = 0; j < batch.warp_blocks; ++j) {
+    const int64_t b = b0 + j * kWarps;
+    if (b >= blocks) break;
+    const float ms = t.ms[b], vs = t.vs[b];
+    const int64_t at = b * kBlock;
+    if (aligned && at + kBlock <= t.numel) {
+      const int64_t o = at + lane * 8;
+      float2 m[4], v[4];
+      moment_values(*reinterpret_cast<const uint2*>(t.mc + o), ms, m);
+      square_values(*reinterpret_cast<const uint2*>(t.vc + o), vs, v);
+      store8<float>(t.m + o, m);
+      store8<float>(t.v + o, v);
+    } else {
+      for (int64_t o = at + lane; o < min(at + kBlock, t.numel); o += 32) {
+        const int c = t.mc[o], d = t.vc[o];
+        const float d2 = (float)(d * d);
+        t.m[o] = (float)(c * abs(c)) * ms;
+        t.v[o] = __fmul_rn(__fmul_rn(d2, d2), vs);
       }
     }
   }
 }
 
-int64_t items_of(int64_t numel) {
-  const int64_t per = (int64_t)kItemBlocks * kBlock;
-  return (numel + per - 1) / per;
+int64_t blocks_of(int64_t numel) { return (numel + kBlock - 1) / kBlock; }
+
+// Blocks per warp: `most` where the tensors have that many for every warp of the GPU four times
+// over, fewer for smaller ones (small launches take as long as one warp's share).
+int warp_blocks(const int64_t* numels, int num_tensors, int sms, int most) {
+  int64_t blocks = 0;
+  for (int i = 0; i < num_tensors; ++i) blocks += blocks_of(numels[i]);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, blocks / (sms * 3 * kWarps * 4)));
+}
+int64_t items_of(int64_t numel, int warp_blocks) {
+  const int64_t per = (int64_t)warp_blocks * kWarps;
+  return (blocks_of(numel) + per - 1) / per;
 }
 
 int check_state(int i, int64_t numel, const int8_t* mc, const float* ms, const uint8_t* vc,
                 const float* vs) {
-  if (numel < 0) return set_error(PT_ERR_SHAPE, "tensor %d has a negative numel", i);
+  if (numel < 0 || numel > (int64_t(1) << 34))
+    return set_error(PT_ERR_SHAPE, "tensor %d: numel must be in [0, 2^34]", i);
   if (numel == 0) return PT_OK;
   const char* what[4] = {"exp_avg codes", "exp_avg scales", "exp_avg_sq codes",
                          "exp_avg_sq scales"};
@@ -301,7 +491,30 @@ int check_state(int i, int64_t numel, const int8_t* mc, const float* ms, const u
   return PT_OK;
 }
 
+template <typename T>
+void launch_step(const Batch& b, const Scalars& k, int64_t items, cudaStream_t s) {
+  const int smem = (int)(sizeof(Stage<T>) * kWarps * kStages);
+  if (cudaFuncSetAttribute(adamw8_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+      cudaSuccess)
+    adamw8_kernel<T><<<(unsigned)items, kThreads, smem, s>>>(b, k);
+}
+
 }  // namespace
+
+// Reads and clears this file's device error word (called by pt_take_device_error).
+int take_adamw8_device_error(int* code);
+int take_adamw8_device_error(int* code) {
+  int v = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_adamw8_error, sizeof(int)) != cudaSuccess ||
+      (v != 0 && cudaMemcpyToSymbol(g_adamw8_error, &zero, sizeof(int)) != cudaSuccess)) {
+    cudaGetLastError();
+    return set_error(PT_ERR_CUDA, "cannot read the device error word");
+  }
+  *code = v;
+  return PT_OK;
+}
+
 }  // namespace pt
 
 using namespace pt;
@@ -335,18 +548,20 @@ int pt_adamw8_step(void* const* params, const void* const* grads, int8_t* const*
     if ((reinterpret_cast<uintptr_t>(params[i]) | reinterpret_cast<uintptr_t>(grads[i])) % elem)
       return set_error(PT_ERR_INVALID_ARGUMENT, "tensor %d is not aligned to its element size", i);
   }
-  int sms = 0;
-  if (int st = current_device_info(nullptr, &sms)) return st;
   const Scalars k{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2),
                   (float)eps, maximize != 0};
   cudaStream_t s = as_stream(stream);
+  int sms = 0;
+  if (int st = current_device_info(nullptr, &sms)) return st;
+  const int per_warp = warp_blocks(numels, num_tensors, sms, kMaxWarpBlocks);
   for (int i = 0; i < num_tensors;) {
     Batch b;
     b.count = 0;
+    b.warp_blocks = per_warp;
     int64_t items = 0;
     for (; i < num_tensors && b.count < kBatch; ++i) {
       if (numels[i] == 0) continue;
-      items += items_of(numels[i]);
+      items += items_of(numels[i], per_warp);
       const double bc1 = 1.0 - std::pow(beta1, (double)steps[i]);
       const double bc2 = 1.0 - std::pow(beta2, (double)steps[i]);
       b.t[b.count++] = Tensor{params[i], grads[i], exp_avg_codes[i], exp_avg_scales[i],
@@ -355,11 +570,10 @@ int pt_adamw8_step(void* const* params, const void* const* grads, int8_t* const*
                               (float)(1.0 - lrs[i] * weight_decays[i])};
     }
     if (b.count == 0) break;
-    const int grid = (int)std::min<int64_t>(items, (int64_t)sms * (2048 / kThreads));
     switch (dtype) {
-      case PT_FLOAT32: adamw8_kernel<float><<<grid, kThreads, 0, s>>>(b, k); break;
-      case PT_FLOAT16: adamw8_kernel<__half><<<grid, kThreads, 0, s>>>(b, k); break;
-      default: adamw8_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(b, k);
+      case PT_FLOAT32: launch_step<float>(b, k, items, s); break;
+      case PT_FLOAT16: launch_step<__half>(b, k, items, s); break;
+      default: launch_step<__nv_bfloat16>(b, k, items, s);
     }
     if (int st = check_launch("pt_adamw8_step")) return st;
   }
@@ -386,19 +600,21 @@ int pt_adamw8_moments(const int8_t* const* exp_avg_codes, const float* const* ex
   }
   int sms = 0;
   if (int st = current_device_info(nullptr, &sms)) return st;
+  const int per_warp = warp_blocks(numels, num_tensors, sms, kMomentWarpBlocks);
   for (int i = 0; i < num_tensors;) {
     MomentBatch b;
     b.count = 0;
+    b.warp_blocks = per_warp;
     int64_t items = 0;
     for (; i < num_tensors && b.count < kBatch; ++i) {
       if (numels[i] == 0) continue;
-      items += items_of(numels[i]);
+      items += items_of(numels[i], per_warp);
       b.t[b.count++] = MomentTensor{exp_avg_codes[i], exp_avg_scales[i], exp_avg_sq_codes[i],
                                     exp_avg_sq_scales[i], exp_avgs[i], exp_avg_sqs[i],
                                     numels[i], items};
     }
     if (b.count == 0) break;
-    const int grid = (int)std::min<int64_t>(items, (int64_t)sms * (2048 / kThreads));
+    const unsigned grid = (unsigned)items;
     moments_kernel<<<grid, kThreads, 0, as_stream(stream)>>>(b);
     if (int st = check_launch("pt_adamw8_moments")) return st;
   }

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 
 #include "common.cuh"
 
@@ -29,34 +30,40 @@ __device__ int g_logit_loss_error = 0;
 
 namespace {
 
-// Vectors in flight per thread as for the cross-entropy kernels, which read the same rows: 8
-// where rows are only read, 4 where dx is written too.
-#ifndef PT_LL_THREADS
-#define PT_LL_THREADS 128
-#endif
-#ifndef PT_LL_TRIPS
-#define PT_LL_TRIPS 4
-#endif
-constexpr int kThreads = PT_LL_THREADS;
-constexpr int kGradTrips = PT_LL_TRIPS;  // unrolled trips per CTA of the gradient
+// Statistics: 128 threads with 8 vectors in flight each, as for the cross-entropy kernels, which
+// read the same rows (0.97 of the HBM peak at 8192 x 128256 bf16; 0.89 with 256 threads).
+constexpr int kThreads = 128;
 constexpr int kUnrollStats = 8;
+// Gradient: 256 threads with 4 vectors in flight, four such trips per CTA (537 us there, 0.99 of
+// the peak; 550 to 590 us with 128 threads, 557 with more or wider trips).
+constexpr int kGradThreads = 256;
 constexpr int kUnrollGrad = 4;
+constexpr int kGradTrips = 4;
 constexpr int kSumThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f;  // log2(e): exp(a) = 2^(a log2(e))
 constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);  // what it lacks
 // How far ex2.approx is below the true value on average (measured over 4 M points of [-20, 0] on
-// B200; its largest error is 1.4e-7). e + e kExpLow, rounded, adds about that much on average.
+// B200; its largest error is 1.4e-7).
 constexpr float kExpLow = 5.05e-8f;
 constexpr float kRaise = 8.0f;  // how far a value may pass the reference: e^8 V stays in range
 constexpr int kErrBadTarget = 2;
 
-// Row r of the [outer, inner] row grid sits at outer index r / inner, inner index r % inner.
+// Row r of the [outer, inner] row grid sits at outer index r / inner, inner index r % inner. One
+// division by a multiplication serves all the tensors that are addressed by the row.
+struct RowIndex {
+  int64_t outer, inner;
+};
+struct RowDiv {
+  FastDiv div;
+  __device__ __forceinline__ RowIndex operator()(int64_t r) const {
+    const uint32_t o = div.div((uint32_t)r);
+    return {o, (uint32_t)r - o * div.d};
+  }
+};
 struct RowGrid {
-  int64_t inner;
   int64_t outer_stride, inner_stride;  // elements
-  __device__ __forceinline__ int64_t offset(int64_t r) const {
-    const int64_t o = r / inner;
-    return o * outer_stride + (r - o * inner) * inner_stride;
+  __device__ __forceinline__ int64_t offset(RowIndex i) const {
+    return i.outer * outer_stride + i.inner * inner_stride;
   }
 };
 
@@ -64,7 +71,8 @@ struct Targets {
   const int64_t* p;
   RowGrid g;
   int64_t ignore;
-  __device__ __forceinline__ int64_t at(int64_t r) const { return p[g.offset(r)]; }
+  RowDiv index;  // of every per-row tensor of the call
+  __device__ __forceinline__ int64_t at(RowIndex i) const { return p[g.offset(i)]; }
 };
 
 // A set of values x as (reference m, sum of e^(x - m)); m = -inf and s = 0 for the empty set.
@@ -133,15 +141,19 @@ struct Running {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
       const float2 t = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm));
-      const float2 y = make_float2(fast_exp2(t.x), fast_exp2(t.y));
-      s = __fadd2_rn(s, __ffma2_rn(y, splat2(kExpLow), y));
+      s = __fadd2_rn(s, make_float2(fast_exp2(t.x), fast_exp2(t.y)));
     }
   }
   __device__ __forceinline__ void add1(float x) {
     raise(x);
-    s.x += fast_exp(x - base());
+    const float d = x - base();
+    s.x += fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
   }
-  __device__ __forceinline__ Stat stat() const { return {m, s.x + s.y}; }
+  // With the exponentials' mean error taken out, of all but the reference's own, which is 1.
+  __device__ __forceinline__ Stat stat() const {
+    const float sum = s.x + s.y;
+    return {m, m == -INFINITY ? sum : fmaf(sum - 1.0f, kExpLow, sum)};
+  }
 };
 
 // log softmax at the value xt. The differences are taken first: m may be as large as the type
@@ -164,12 +176,17 @@ template <typename T> __device__ __forceinline__ int head_elems(const T* p, int6
   return (int64_t)h < vocab ? h : (int)vocab;
 }
 
-// The part of a row that split `k` of `n` takes: whole 16-byte vectors [v0, v1) of the aligned
+// The part of a row that split `k` of `n` (or of 2^log2_n) takes: whole 16-byte vectors [v0, v1) of the aligned
 // body, the unaligned head with the first split and the tail with the last.
 struct Part {
   int64_t v0, v1;
   __device__ __forceinline__ Part(int64_t nvec, int k, int n) {
     const int64_t per = (nvec + n - 1) / n;
+    v0 = min(nvec, per * k);
+    v1 = min(nvec, v0 + per);
+  }
+  __device__ __forceinline__ Part(int64_t nvec, int k, int log2_n, std::nullptr_t) {
+    const int64_t per = (nvec + (1 << log2_n) - 1) >> log2_n;
     v0 = min(nvec, per * k);
     v1 = min(nvec, v0 + per);
   }
@@ -214,13 +231,14 @@ stats_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows,
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
     const int64_t r = splits == 1 ? it : it / splits;
     const int k = (int)(it - r * splits);
-    const int64_t t = tg.at(r);
+    const RowIndex index = tg.index(r);
+    const int64_t t = tg.at(index);
     const RowKind kind = row_kind(t, tg.ignore, vocab);
     if (kind != kRowUsed) {
       if (splits == 1 && threadIdx.x == 0) out.store(r, kind, Stat{0.0f, 1.0f}, 0.0f);
       continue;
     }
-    const T* row = logits + lg.offset(r);
+    const T* row = logits + lg.offset(index);
     const float xt = splits == 1 && threadIdx.x == 0 ? to_float(row[t]) : 0.0f;
     const int head = head_elems(row, vocab);
     const T* body = row + head;
@@ -268,12 +286,13 @@ finish_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows
   constexpr int kWarps = kThreads / 32;
   for (int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows;
        r += (int64_t)gridDim.x * kWarps) {
-    const int64_t t = tg.at(r);
+    const RowIndex index = tg.index(r);
+    const int64_t t = tg.at(index);
     const RowKind kind = row_kind(t, tg.ignore, vocab);
     Stat v{-INFINITY, 0.0f};
     float xt = 0.0f;
     if (kind == kRowUsed) {
-      xt = to_float(logits[lg.offset(r) + t]);
+      xt = to_float(logits[lg.offset(index) + t]);
       for (int k = lane; k < splits; k += 32) v.m = fmaxf(v.m, part[r * splits + k].m);
       v.m = warp_max(v.m);
       for (int k = lane; k < splits; k += 32) v.s += sum_at(part[r * splits + k], v.m);
@@ -289,7 +308,7 @@ finish_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows
 // at 8192 x 128256 bf16 with a third of the rows ignored). Rows are visited from the last to
 // the first: the forward read the last ones last, so they are still in L2.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kGradThreads)
 grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, int64_t vocab,
             int splits, const float2* __restrict__ stats, const float* __restrict__ coef,
             RowGrid cg, const float* __restrict__ grad, T* __restrict__ dlogits, RowGrid dg) {
@@ -300,9 +319,10 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
     const int64_t rr = splits == 1 ? it : it / splits;
     const int k = (int)(it - rr * splits);
     const int64_t r = rows - 1 - rr;
-    const T* row = logits + lg.offset(r);
-    T* drow = dlogits + dg.offset(r);
-    const int64_t t = tg.at(r);
+    const RowIndex index = tg.index(r);
+    const int64_t t = tg.at(index);
+    const T* row = logits + lg.offset(index);
+    T* drow = dlogits + dg.offset(index);
     const bool used = row_kind(t, tg.ignore, vocab) == kRowUsed;
     const int head = head_elems(row, vocab);
     const T* body = row + head;
@@ -313,14 +333,14 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
     if (!used) {
       const uint4 z = make_uint4(0, 0, 0, 0);
       if (k == 0 && (int)threadIdx.x < head) drow[threadIdx.x] = from_float<T>(0.0f);
-      for (int64_t v = p.v0 + threadIdx.x; v < p.v1; v += kThreads) st_stream(dbody + v * V, z);
+      for (int64_t v = p.v0 + threadIdx.x; v < p.v1; v += kGradThreads) st_stream(dbody + v * V, z);
       if (k == splits - 1)
-        for (int64_t c = tail + threadIdx.x; c < vocab; c += kThreads)
+        for (int64_t c = tail + threadIdx.x; c < vocab; c += kGradThreads)
           drow[c] = from_float<T>(0.0f);
       continue;
     }
     const float2 st = stats[r];
-    const float c = coef[cg.offset(r)] * scale;
+    const float c = coef[cg.offset(index)] * scale;
     const float a = -c * st.y, nm = -st.x;
     auto one = [&](int64_t col) {
       const float e = fast_exp(to_float(row[col]) + nm);
@@ -332,7 +352,8 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
       unpack<T>(raw, x);
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const float2 y = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2));
+        const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2),
+                                    splat2(kLog2e));
         x[e] = fast_exp2(y.x);
         x[e + 1] = fast_exp2(y.y);
       }
@@ -348,16 +369,16 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
     };
     if (k == 0 && (int)threadIdx.x < head) one(threadIdx.x);
     int64_t v = p.v0 + threadIdx.x;
-    for (; v + (kUnrollGrad - 1) * kThreads < p.v1; v += kUnrollGrad * kThreads) {
+    for (; v + (kUnrollGrad - 1) * kGradThreads < p.v1; v += kUnrollGrad * kGradThreads) {
       uint4 raw[kUnrollGrad];
 #pragma unroll
-      for (int u = 0; u < kUnrollGrad; ++u) raw[u] = ld_stream(body + (v + u * kThreads) * V);
+      for (int u = 0; u < kUnrollGrad; ++u) raw[u] = ld_stream(body + (v + u * kGradThreads) * V);
 #pragma unroll
-      for (int u = 0; u < kUnrollGrad; ++u) vec(raw[u], v + u * kThreads);
+      for (int u = 0; u < kUnrollGrad; ++u) vec(raw[u], v + u * kGradThreads);
     }
-    for (; v < p.v1; v += kThreads) vec(ld_stream(body + v * V), v);
+    for (; v < p.v1; v += kGradThreads) vec(ld_stream(body + v * V), v);
     if (k == splits - 1)
-      for (int64_t col = tail + threadIdx.x; col < vocab; col += kThreads) one(col);
+      for (int64_t col = tail + threadIdx.x; col < vocab; col += kGradThreads) one(col);
   }
 }
 
@@ -377,13 +398,14 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
 // bits: the sum of differences, not a difference of long sums. One CTA per sequence.
 __global__ void __launch_bounds__(256)
 pair_ratio_kernel(const double* __restrict__ logps, const float* __restrict__ ref, RowGrid rg,
-                  Targets tg, double* __restrict__ ratio) {
+                  Targets tg, int64_t inner, double* __restrict__ ratio) {
   __shared__ double red[8];
-  const int64_t q = blockIdx.x, inner = tg.g.inner;
+  const int64_t q = blockIdx.x;
   double s = 0.0;
+#pragma unroll 2
   for (int64_t i = threadIdx.x; i < inner; i += 256) {
-    const int64_t r = q * inner + i;
-    if (tg.at(r) != tg.ignore) s += logps[r] - (double)ref[rg.offset(r)];
+    const RowIndex at{q, i};
+    if (tg.at(at) != tg.ignore) s += logps[q * inner + i] - (double)ref[rg.offset(at)];
   }
   s = block_sum(s, red);
   if (threadIdx.x == 0) ratio[q] = s;
@@ -420,16 +442,16 @@ pair_loss_kernel(const double* __restrict__ ratio, int64_t pairs, double beta, d
 // is 1 / (positions with a target); over sequences 1 / (such positions of q * sequences that
 // have any). One CTA of 32 warps.
 __global__ void __launch_bounds__(kSumThreads)
-policy_weight_kernel(Targets tg, int64_t outer, int by_sequence, double* __restrict__ weight) {
+policy_weight_kernel(Targets tg, int64_t outer, int64_t inner, int by_sequence,
+                     double* __restrict__ weight) {
   __shared__ double red[kSumThreads / 32];
   __shared__ double total;
-  const int64_t inner = tg.g.inner;
   if (by_sequence) {
     const int lane = threadIdx.x & 31;
     double some = 0.0;
     for (int64_t q = threadIdx.x >> 5; q < outer; q += kSumThreads / 32) {
       double n = 0.0;
-      for (int64_t i = lane; i < inner; i += 32) n += tg.at(q * inner + i) != tg.ignore;
+      for (int64_t i = lane; i < inner; i += 32) n += tg.at({q, i}) != tg.ignore;
       n = warp_sum(n);
       if (lane == 0) {
         weight[q] = n;
@@ -443,8 +465,9 @@ policy_weight_kernel(Targets tg, int64_t outer, int by_sequence, double* __restr
       weight[q] = weight[q] > 0.0 ? 1.0 / (weight[q] * total) : 0.0;
   } else {
     double n = 0.0;
+#pragma unroll 4
     for (int64_t r = threadIdx.x; r < outer * inner; r += kSumThreads)
-      n += tg.at(r) != tg.ignore;
+      n += tg.at(tg.index(r)) != tg.ignore;
     n = block_sum(n, red);
     if (threadIdx.x == 0) total = n;
     __syncthreads();
@@ -471,11 +494,11 @@ struct PolicyTerms {
 struct PolicyRow {
   float old, adv, ref;
   double weight;
-  __device__ __forceinline__ void load(const PolicyTerms& p, int64_t r, int64_t inner) {
-    old = p.old[p.og.offset(r)];
-    adv = p.adv[p.ag.offset(r)];
-    ref = p.ref != nullptr ? p.ref[p.rg.offset(r)] : 0.0f;
-    weight = p.weight[r / inner];
+  __device__ __forceinline__ void load(const PolicyTerms& p, RowIndex i) {
+    old = p.old[p.og.offset(i)];
+    adv = p.adv[p.ag.offset(i)];
+    ref = p.ref != nullptr ? p.ref[p.rg.offset(i)] : 0.0f;
+    weight = p.weight[i.outer];
   }
   // max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
   // derivative to lp: -A r where the unclipped term is the larger one, and kl (1 - e^g). The
@@ -505,9 +528,10 @@ policy_row_kernel(const double* __restrict__ logps, Targets tg, int64_t rows, Po
        r += (int64_t)gridDim.x * kThreads) {
     double term = 0.0;
     float coef = 0.0f;
-    if (tg.at(r) != tg.ignore) {
+    const RowIndex index = tg.index(r);
+    if (tg.at(index) != tg.ignore) {
       PolicyRow row;
-      row.load(p, r, tg.g.inner);
+      row.load(p, index);
       row.term(p, logps[r], term, coef);
     }
     p.term[r] = term;
@@ -539,19 +563,14 @@ policy_sum_kernel(const double* __restrict__ term, int64_t rows, const double* _
 // asynchronous stores into each other's shared memory, which complete on the receiver's barrier:
 // one thread waits for it, not the whole cluster. Several clusters share an SM, so one row's
 // loads overlap another's arithmetic and stores.
-#ifndef PT_POLICY_BLOCKS
-#define PT_POLICY_BLOCKS 4
-#endif
-#ifndef PT_POLICY_THREADS
-#define PT_POLICY_THREADS 256
-#endif
-#ifndef PT_POLICY_SLICE
-#define PT_POLICY_SLICE 32
-#endif
-constexpr int kFusedThreads = PT_POLICY_THREADS;
+// 128 threads and slices of up to 32 KB, seven CTAs per SM: 633 us at 8192 x 128256 bf16 with 35 %
+// of the rows ignored (680 us with 256 threads and 64 KB, 715 with 64 threads and 16 KB), against
+// 753 us for statistics and gradient in two passes.
+constexpr int kFusedThreads = 128;
+constexpr int kFusedBlocks = 7;
 constexpr int kFusedWarps = kFusedThreads / 32;
 constexpr int kMaxCluster = 8;  // the portable cluster size
-constexpr int kSliceBytes = PT_POLICY_SLICE * 1024;
+constexpr int kSliceBytes = 32 * 1024;
 constexpr int kMaxSliceBytes = 192 * 1024;
 constexpr int kErrWait = kDeviceErrWaitTimeout;
 
@@ -581,7 +600,8 @@ __device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar) {
   for (;;) {
     uint32_t done;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
         " selp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(smem_addr(bar))
@@ -592,11 +612,12 @@ __device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kFusedThreads, PT_POLICY_BLOCKS)
+__global__ void __launch_bounds__(kFusedThreads, kFusedBlocks)
 policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t vocab,
-                   int cluster, PolicyTerms p, float grad, RowOut out, T* __restrict__ dlogits,
-                   RowGrid dg) {
+                   int log2_cluster, PolicyTerms p, float grad, RowOut out,
+                   T* __restrict__ dlogits, RowGrid dg) {
   constexpr int V = Vec16<T>::N;
+  const int cluster = 1 << log2_cluster;
   extern __shared__ __align__(16) unsigned char slice[];
   __shared__ uint64_t bar[kFusedWarps];
   __shared__ uint64_t peer_bar;
@@ -605,15 +626,16 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
   __shared__ float3 shared_row;  // reference, 1 / s, coefficient
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cluster > 1 ? (int)cluster_rank() : 0;
-  const int64_t r = blockIdx.x / (unsigned)cluster;
-  const T* row = logits + lg.offset(r);
-  T* drow = dlogits + dg.offset(r);
-  const int64_t t = tg.at(r);
+  const int64_t r = blockIdx.x >> log2_cluster;
+  const RowIndex index = tg.index(r);
+  const int64_t t = tg.at(index);
+  const T* row = logits + lg.offset(index);
+  T* drow = dlogits + dg.offset(index);
   const RowKind kind = row_kind(t, tg.ignore, vocab);
   const int head = head_elems(row, vocab);
   const int64_t nvec = (vocab - head) / V;
   const int64_t tail = head + nvec * V;
-  const Part part(nvec, rank, cluster);
+  const Part part(nvec, rank, log2_cluster, nullptr);
   const int n = (int)(part.v1 - part.v0);
   const T* body = row + head + part.v0 * V;
   T* dbody = drow + head + part.v0 * V;
@@ -658,7 +680,7 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
   PolicyRow terms;
   if (tid == 0) {
     xt = to_float(row[t]);
-    terms.load(p, r, tg.g.inner);
+    terms.load(p, index);
   }
   const float xe = edge >= 0 ? to_float(row[edge]) : 0.0f;
   Running acc;
@@ -724,7 +746,7 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
     unpack<T>(lds128(slice + (size_t)u * 16), x);
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
-      const float2 y = log2_scaled(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2));
+      const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2), splat2(kLog2e));
       const float2 d = __fmul2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), a2);
       x[e] = d.x;
       x[e + 1] = d.y;
@@ -737,13 +759,13 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
 // dx *= grad / expected, unless they are equal.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-rescale_kernel(T* __restrict__ dlogits, RowGrid dg, int64_t rows, int64_t vocab,
+rescale_kernel(T* __restrict__ dlogits, RowGrid dg, RowDiv index, int64_t rows, int64_t vocab,
                const float* __restrict__ grad, float expected) {
   constexpr int V = Vec16<T>::N;
   if (*grad == expected) return;
   const float f = *grad / expected;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    T* row = dlogits + dg.offset(r);
+    T* row = dlogits + dg.offset(index(r));
     const int head = head_elems(row, vocab);
     const int64_t nvec = (vocab - head) / V;
     for (int64_t v = threadIdx.x; v < nvec; v += kThreads) {
@@ -785,8 +807,8 @@ int64_t workspace_bytes(int64_t rows, int64_t outer, int splits) {
 
 int check_sizes(int64_t vocab, int64_t outer, int64_t inner, int64_t* rows) {
   if (outer < 0 || inner < 0 || __builtin_mul_overflow(outer, inner, rows) ||
-      *rows > (int64_t(1) << 40))
-    return set_error(PT_ERR_SHAPE, "outer and inner must be >= 0 and their product below 2^40");
+      *rows > INT32_MAX || outer > INT32_MAX || inner > INT32_MAX)
+    return set_error(PT_ERR_SHAPE, "outer, inner and their product must be in [0, 2^31)");
   if (vocab < 1 || vocab > (int64_t(1) << 31))
     return set_error(PT_ERR_SHAPE, "vocab must be in [1, 2^31] (got %lld)", (long long)vocab);
   return PT_OK;
@@ -809,8 +831,8 @@ int check_rows(Rows& g, const void* logits, int64_t vocab, int64_t outer, int64_
   g.outer = outer;
   g.inner = inner > 0 ? inner : 1;
   g.splits = split_count(g.rows, vocab, elem, g.sms);
-  g.lg = RowGrid{g.inner, lo, li};
-  g.tg = Targets{targets, RowGrid{g.inner, to, ti}, ignore};
+  g.lg = RowGrid{lo, li};
+  g.tg = Targets{targets, RowGrid{to, ti}, ignore, RowDiv{FastDiv((uint32_t)g.inner)}};
   return PT_OK;
 }
 
@@ -910,11 +932,11 @@ int check_policy(Rows& g, Workspace& w, PolicyTerms& p, const PolicyInputs& in,
   if (int st = check_optional(coef, "coef", g.rows)) return st;
   if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
   p.old = in.old;
-  p.og = RowGrid{g.inner, in.oo, in.oi};
+  p.og = RowGrid{in.oo, in.oi};
   p.adv = in.adv;
-  p.ag = RowGrid{g.inner, in.ao, in.ai};
+  p.ag = RowGrid{in.ao, in.ai};
   p.ref = in.ref;
-  p.rg = RowGrid{g.inner, in.ro, in.ri};
+  p.rg = RowGrid{in.ro, in.ri};
   p.weight = w.seq;
   p.low = (float)(1.0 - in.low);
   p.high = (float)(1.0 + in.high);
@@ -960,8 +982,10 @@ int launch_policy_grad(const Rows& g, const void* logits, int cluster, const Pol
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    int log2_cluster = 0;
+    while (1 << log2_cluster < cluster) ++log2_cluster;
     e = cudaLaunchKernelEx(&cfg, policy_grad_kernel<T>, static_cast<const T*>(logits), g.lg, g.tg,
-                           g.vocab, cluster, p, grad, out, static_cast<T*>(dlogits), dg);
+                           g.vocab, log2_cluster, p, grad, out, static_cast<T*>(dlogits), dg);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1047,27 +1071,28 @@ int pt_token_logps_bwd(const void* logits, int64_t vocab, int64_t outer, int64_t
   if (int st = check_same_rows(g, logits, logits_outer_stride, logits_inner_stride, dlogits,
                                dlogits_outer_stride, dlogits_inner_stride, dtype_size(dtype)))
     return st;
-  const RowGrid cg{g.inner, coef_outer_stride, coef_inner_stride};
-  const RowGrid dg{g.inner, dlogits_outer_stride, dlogits_inner_stride};
+  const RowGrid cg{coef_outer_stride, coef_inner_stride};
+  const RowGrid dg{dlogits_outer_stride, dlogits_inner_stride};
   const float2* st2 = reinterpret_cast<const float2*>(stats);
-  const int64_t vecs = vocab * dtype_size(dtype) / 16;
-  const int splits =
-      (int)std::max<int64_t>(1, vecs / (kThreads * kUnrollGrad * kGradTrips));
+  // kGradTrips unrolled trips per CTA, fewer (down to one) while that leaves SMs without eight CTAs.
+  const int64_t trips = vocab * dtype_size(dtype) / 16 / (kGradThreads * kUnrollGrad);
+  const int64_t spread = std::min(trips, ((int64_t)g.sms * 8 + g.rows - 1) / g.rows);
+  const int splits = (int)std::max<int64_t>({1, trips / kGradTrips, spread});
   const int grid = grid_of(g.rows * splits);
   cudaStream_t s = as_stream(stream);
   switch (dtype) {
     case PT_FLOAT32:
-      grad_kernel<float><<<grid, kThreads, 0, s>>>(static_cast<const float*>(logits), g.lg, g.tg,
+      grad_kernel<float><<<grid, kGradThreads, 0, s>>>(static_cast<const float*>(logits), g.lg, g.tg,
                                                    g.rows, vocab, splits, st2, coef, cg, grad,
                                                    static_cast<float*>(dlogits), dg);
       break;
     case PT_FLOAT16:
-      grad_kernel<__half><<<grid, kThreads, 0, s>>>(static_cast<const __half*>(logits), g.lg,
+      grad_kernel<__half><<<grid, kGradThreads, 0, s>>>(static_cast<const __half*>(logits), g.lg,
                                                     g.tg, g.rows, vocab, splits, st2, coef, cg,
                                                     grad, static_cast<__half*>(dlogits), dg);
       break;
     default:
-      grad_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(
+      grad_kernel<__nv_bfloat16><<<grid, kGradThreads, 0, s>>>(
           static_cast<const __nv_bfloat16*>(logits), g.lg, g.tg, g.rows, vocab, splits, st2,
           coef, cg, grad, static_cast<__nv_bfloat16*>(dlogits), dg);
   }
@@ -1098,19 +1123,15 @@ int pt_preference_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int
   if (int st = check_optional(stats, "stats", g.rows)) return st;
   if (int st = check_optional(rewards, "rewards", outer)) return st;
   if (int st = check_optional(coef, "coef", outer)) return st;
-  if (outer > INT32_MAX) return set_error(PT_ERR_SHAPE, "too many sequences");
   Workspace w;
   if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
   cudaStream_t s = as_stream(stream);
   row_stats(g, logits, dtype, w.part, RowOut{reinterpret_cast<float2*>(stats), nullptr, w.logps},
             s);
-  if (outer > 0) {
-    Targets tg = g.tg;
-    tg.g.inner = inner;  // zero positions sum to zero
+  if (outer > 0)
     pair_ratio_kernel<<<(unsigned)outer, 256, 0, s>>>(
-        w.logps, reference, RowGrid{g.inner, reference_outer_stride, reference_inner_stride}, tg,
+        w.logps, reference, RowGrid{reference_outer_stride, reference_inner_stride}, g.tg, inner,
         w.seq);
-  }
   pair_loss_kernel<<<1, kSumThreads, 0, s>>>(w.seq, outer / 2, beta, label_smoothing, loss,
                                              rewards, coef);
   return check_launch("pt_preference_loss_fwd");
@@ -1143,7 +1164,7 @@ int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t
   row_stats(g, logits, dtype, w.part, RowOut{reinterpret_cast<float2*>(stats), logps, w.logps},
             s);
   const int64_t sequences = g.rows > 0 ? outer : 0;
-  policy_weight_kernel<<<1, kSumThreads, 0, s>>>(g.tg, sequences, by_sequence, w.seq);
+  policy_weight_kernel<<<1, kSumThreads, 0, s>>>(g.tg, sequences, g.inner, by_sequence, w.seq);
   if (g.rows > 0)
     policy_row_kernel<<<grid_of((g.rows + kThreads - 1) / kThreads, g.sms, 2048 / kThreads),
                         kThreads, 0, s>>>(w.logps, g.tg, g.rows, p);
@@ -1197,9 +1218,9 @@ int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_
                      (long long)vocab);
   cudaStream_t s = as_stream(stream);
   const int64_t sequences = g.rows > 0 ? outer : 0;
-  policy_weight_kernel<<<1, kSumThreads, 0, s>>>(g.tg, sequences, by_sequence, w.seq);
+  policy_weight_kernel<<<1, kSumThreads, 0, s>>>(g.tg, sequences, g.inner, by_sequence, w.seq);
   if (g.rows > 0) {
-    const RowGrid dg{g.inner, dlogits_outer_stride, dlogits_inner_stride};
+    const RowGrid dg{dlogits_outer_stride, dlogits_inner_stride};
     const RowOut out{reinterpret_cast<float2*>(stats), logps, nullptr};
     int st;
     switch (dtype) {
@@ -1233,20 +1254,21 @@ int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t 
   if (int st = check_device_ptr(grad, "grad")) return st;
   int sms = 0;
   if (int st = current_device_info(nullptr, &sms)) return st;
-  const RowGrid dg{inner, dlogits_outer_stride, dlogits_inner_stride};
+  const RowGrid dg{dlogits_outer_stride, dlogits_inner_stride};
+  const RowDiv index{FastDiv((uint32_t)inner)};
   const int grid = grid_of(rows, sms, 2048 / kThreads);
   cudaStream_t s = as_stream(stream);
   switch (dtype) {
     case PT_FLOAT32:
-      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<float*>(dlogits), dg, rows, vocab, grad,
-                                               (float)expected);
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<float*>(dlogits), dg, index, rows, vocab,
+                                               grad, (float)expected);
       break;
     case PT_FLOAT16:
-      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__half*>(dlogits), dg, rows, vocab,
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__half*>(dlogits), dg, index, rows, vocab,
                                                grad, (float)expected);
       break;
     default:
-      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__nv_bfloat16*>(dlogits), dg, rows,
+      rescale_kernel<<<grid, kThreads, 0, s>>>(static_cast<__nv_bfloat16*>(dlogits), dg, index, rows,
                                                vocab, grad, (float)expected);
   }
   return check_launch("pt_rescale_logits_grad");

@@ -47,10 +47,12 @@
 namespace pt {
 
 // Read and clear the device error words of the fused SwiGLU GEMM (swiglu_gemm.cu), of the
-// cross-entropy kernels (cross_entropy.cu) and of the logit losses (logit_loss.cu).
+// cross-entropy kernels (cross_entropy.cu), of the logit losses (logit_loss.cu) and of the 8-bit
+// AdamW step (adamw8.cu).
 int take_gemm_device_error(int* code);
 int take_ce_device_error(int* code);
 int take_logit_loss_device_error(int* code);
+int take_adamw8_device_error(int* code);
 
 // Device-side error word of this library on each device (0 = none). Kernels that give up
 // on a bounded wait record kDeviceErrWaitTimeout here; pt_take_device_error reads it.
@@ -1668,11 +1670,14 @@ int pt_take_device_error(int* code) {
                        cudaGetErrorString(e));
     }
   }
-  int gemm_value = 0, ce_value = 0, loss_value = 0;
+  int gemm_value = 0, ce_value = 0, loss_value = 0, adamw8_value = 0;
   if (int st = take_gemm_device_error(&gemm_value)) return st;
   if (int st = take_ce_device_error(&ce_value)) return st;
   if (int st = take_logit_loss_device_error(&loss_value)) return st;
-  *code = value != 0 ? value : gemm_value != 0 ? gemm_value : ce_value != 0 ? ce_value : loss_value;
+  if (int st = take_adamw8_device_error(&adamw8_value)) return st;
+  *code = 0;
+  for (int v : {value, gemm_value, ce_value, loss_value, adamw8_value})
+    if (*code == 0) *code = v;
   return ok();
 }
 

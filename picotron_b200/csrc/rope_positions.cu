@@ -21,8 +21,12 @@
 namespace pt {
 namespace {
 
+// 128 threads (64 and 256 took 1.1 and 1.2 times as long at B 8, S 2048, 32 + 8 heads of 128,
+// bf16: 54 us, 0.95 of the HBM peak). Units in flight per thread: five where a token has that
+// many, as there, else three (54 against 60 us there; 3.1 against 3.9 us for 32 decoded tokens).
 constexpr int kThreads = 128;
-constexpr int kUnits = 4;                      // units in flight per thread
+constexpr int kManyUnits = 5;
+constexpr int kFewUnits = 3;
 constexpr int kTableBytes = 32 * 1024;         // of shared memory for a CTA's angles
 constexpr int kMaxTokens = 16;                 // tokens per CTA
 
@@ -39,9 +43,8 @@ struct Geom {
   uint32_t rot_units;
   uint32_t token_units;      // heads * head_units
   uint32_t tokens_per_cta;
-  uint32_t S;
-  int64_t tokens;            // B * S
-  FastDiv div_token, div_head;
+  uint32_t tokens;           // B * S
+  FastDiv div_token, div_head, div_s, div_half;
   float scale, sign;
 };
 
@@ -87,17 +90,32 @@ template <typename T, int N> struct Pack {
 
 // A unit is N elements (two single ones for N = 1 interleaved), or for rotated rotate-half
 // units N elements of each half.
-template <typename T, int N, bool kRotateHalf>
+// kOne: a CTA takes one token, whose rows' addresses are the same for all its threads.
+template <typename T, int N, bool kRotateHalf, bool kOne, int kUnits>
 __global__ void __launch_bounds__(kThreads)
 rope_positions_kernel(const __grid_constant__ Geom g) {
   extern __shared__ float2 table[];  // [tokens_per_cta][half] (c, s)
   constexpr bool kPairLoads = !kRotateHalf && N == 1;
   constexpr int kSpan = kPairLoads ? 2 : N;  // elements from one unit's start to the next
-  const int64_t token0 = (int64_t)blockIdx.x * g.tokens_per_cta;
-  const uint32_t count = (uint32_t)min((int64_t)g.tokens_per_cta, g.tokens - token0);
+  const uint32_t token0 = kOne ? blockIdx.x : blockIdx.x * g.tokens_per_cta;
+  const uint32_t count = kOne ? 1u : min(g.tokens_per_cta, g.tokens - token0);
   const uint32_t total = count * g.token_units;
-  const T* X[2] = {static_cast<const T*>(g.x[0]), static_cast<const T*>(g.x[1])};
-  T* O[2] = {static_cast<T*>(g.out[0]), static_cast<T*>(g.out[1])};
+
+  struct Token {
+    const T* x[2];
+    T* out[2];
+  };
+  auto token_at = [&](uint32_t tok) {
+    const uint32_t b = g.div_s.div(token0 + tok), s = token0 + tok - b * g.div_s.d;
+    Token t;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t.x[i] = static_cast<const T*>(g.x[i]) + (int64_t)b * g.xb[i] + (int64_t)s * g.xs[i];
+      t.out[i] = static_cast<T*>(g.out[i]) + (int64_t)b * g.ob[i] + (int64_t)s * g.os[i];
+    }
+    return t;
+  };
+  const Token one = kOne ? token_at(0) : Token{};
 
   struct Where {
     const T* x;
@@ -106,23 +124,23 @@ rope_positions_kernel(const __grid_constant__ Geom g) {
     bool rotated;
   };
   auto where = [&](uint32_t u) {
-    const uint32_t tok = g.div_token.div(u);
-    const uint32_t in = u - tok * g.token_units;
+    uint32_t tok = 0, in = u;
+    if (!kOne) {
+      tok = g.div_token.div(u);
+      in = u - tok * g.token_units;
+    }
+    const Token t = kOne ? one : token_at(tok);
     const uint32_t h = g.div_head.div(in);
     const uint32_t j = in - h * g.head_units;
-    const int64_t token = token0 + tok;
-    const int64_t b = token / g.S, s = token - b * g.S;
     const bool second = h >= g.heads0;
     const int64_t hh = second ? h - g.heads0 : h;
     Where w;
     w.rotated = j < g.rot_units;
     // Copied units of a rotate-half head start behind both halves.
-    const int64_t d =
+    const uint32_t d =
         kRotateHalf ? (w.rotated ? j * kSpan : 2 * g.half + (j - g.rot_units) * kSpan) : j * kSpan;
-    w.x = second ? X[1] + b * g.xb[1] + hh * g.xh[1] + s * g.xs[1] + d
-                 : X[0] + b * g.xb[0] + hh * g.xh[0] + s * g.xs[0] + d;
-    w.out = second ? O[1] + b * g.ob[1] + hh * g.oh[1] + s * g.os[1] + d
-                   : O[0] + b * g.ob[0] + hh * g.oh[0] + s * g.os[0] + d;
+    w.x = (second ? t.x[1] + hh * g.xh[1] : t.x[0] + hh * g.xh[0]) + d;
+    w.out = (second ? t.out[1] + hh * g.oh[1] : t.out[0] + hh * g.oh[0]) + d;
     w.table = tok * g.half + j * (kRotateHalf ? N : kSpan / 2);
     return w;
   };
@@ -184,9 +202,8 @@ rope_positions_kernel(const __grid_constant__ Geom g) {
     }
   }
   for (uint32_t i = threadIdx.x; i < count * g.half; i += kThreads) {
-    const uint32_t tok = i / g.half, p = i - tok * g.half;
-    const int64_t token = token0 + tok;
-    const int64_t b = token / g.S, s = token - b * g.S;
+    const uint32_t tok = kOne ? 0 : g.div_half.div(i), p = i - tok * g.half;
+    const uint32_t b = g.div_s.div(token0 + tok), s = token0 + tok - b * g.div_s.d;
     const double a = (double)g.positions[b * g.pb + s * g.ps] * g.inv_freq[p];
     // a less whole turns, with 2 pi as a sum of two 64-bit numbers: exact to 64 bits for any a
     // whose turns are whole numbers in 64 bits, where a fraction of a / (2 pi) loses |a| 2^-53.
@@ -250,18 +267,25 @@ int launch(Geom& g, int64_t D, int64_t R, bool rh, cudaStream_t s) {
   g.head_units = (uint32_t)(g.rot_units + copied);
   g.token_units = (uint32_t)units;
   // Enough tokens per CTA to give every thread its units in flight, as far as the angles fit.
-  const int64_t want = std::max<int64_t>(1, kThreads * kUnits / units);
+  const int64_t want = std::max<int64_t>(1, kThreads * kFewUnits / units);
   const int64_t room = std::max<int64_t>(1, kTableBytes / ((int64_t)g.half * 8));
-  g.tokens_per_cta = (uint32_t)std::min<int64_t>({want, room, kMaxTokens, g.tokens});
+  g.tokens_per_cta = (uint32_t)std::min<int64_t>({want, room, kMaxTokens, (int64_t)g.tokens});
   g.div_token = FastDiv(g.token_units);
   g.div_head = FastDiv(g.head_units);
-  const int64_t grid = (g.tokens + g.tokens_per_cta - 1) / g.tokens_per_cta;
-  if (grid > INT32_MAX) return set_error(PT_ERR_SHAPE, "too many tokens");
+  g.div_half = FastDiv(g.half);
+  const unsigned grid = (g.tokens + g.tokens_per_cta - 1) / g.tokens_per_cta;
   const size_t smem = (size_t)g.tokens_per_cta * g.half * sizeof(float2);
-  if (rh)
-    rope_positions_kernel<T, N, true><<<(unsigned)grid, kThreads, smem, s>>>(g);
-  else
-    rope_positions_kernel<T, N, false><<<(unsigned)grid, kThreads, smem, s>>>(g);
+  auto kernel = rh ? rope_positions_kernel<T, N, true, false, kFewUnits>
+                   : rope_positions_kernel<T, N, false, false, kFewUnits>;
+  if (g.tokens_per_cta == 1) {
+    if (units > kThreads * kFewUnits)
+      kernel = rh ? rope_positions_kernel<T, N, true, true, kManyUnits>
+                  : rope_positions_kernel<T, N, false, true, kManyUnits>;
+    else
+      kernel = rh ? rope_positions_kernel<T, N, true, true, kFewUnits>
+                  : rope_positions_kernel<T, N, false, true, kFewUnits>;
+  }
+  kernel<<<grid, kThreads, smem, s>>>(g);
   return check_launch("pt_rope_positions");
 }
 
@@ -322,6 +346,8 @@ int pt_rope_positions(const void* q, const int64_t q_strides[4], void* q_out,
   if (position_batch_stride < 0 || position_stride < 0)
     return set_error(PT_ERR_SHAPE, "negative position stride");
   if (B * S == 0 || q_sizes[1] + k_sizes[1] == 0) return ok();
+  if (B * S > INT32_MAX || q_sizes[1] + k_sizes[1] > INT32_MAX)
+    return set_error(PT_ERR_SHAPE, "B * S and the heads together must be below 2^31");
   for (const Side& t : sides) {
     if (t.sizes[1] == 0) continue;
     if (int st = check_device_ptr(t.x, "x")) return st;
@@ -349,8 +375,8 @@ int pt_rope_positions(const void* q, const int64_t q_strides[4], void* q_out,
   g.inv_freq = inv_freq;
   g.heads0 = (uint32_t)q_sizes[1];
   g.heads = (uint32_t)(q_sizes[1] + k_sizes[1]);
-  g.S = (uint32_t)S;
-  g.tokens = B * S;
+  g.tokens = (uint32_t)(B * S);
+  g.div_s = FastDiv((uint32_t)S);
   g.scale = (float)scale;
   g.sign = backward ? -1.0f : 1.0f;
   const bool rh = layout == PT_ROPE_ROTATE_HALF;

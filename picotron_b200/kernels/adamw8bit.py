@@ -30,25 +30,25 @@ def _scales(numel: int) -> int:
     return (numel + BLOCK - 1) // BLOCK
 
 
-def _check_states(lists: Sequence[Sequence[Tensor]], numels: Sequence[int] | None):
-    """Validate the four state lists; returns (device, numels)."""
+def _addresses(name: str, tensors: Sequence[Tensor], sizes: Sequence[int], dtype: torch.dtype,
+               device: int) -> list[int]:
+    """Data addresses of contiguous tensors with these sizes, dtype and CUDA device."""
 
-    if len(lists[0]) == 0:
-        return None, []
-    device = lists[0][0].device
-    sizes = [t.numel() for t in lists[0]]
-    if numels is not None and sizes != list(numels):
-        raise TritonAdamWUnavailable("exp_avg codes must have one element per parameter element.")
-    for values, (name, dtype) in zip(lists, _STATE.items()):
-        if len(values) != len(sizes):
-            raise TritonAdamWUnavailable("all tensor lists must have the same length.")
-        for t, n in zip(values, sizes):
-            if t.dtype != dtype or t.device != device or not t.is_contiguous():
-                raise TritonAdamWUnavailable(
-                    f"{name} must be contiguous {dtype} tensors on one device.")
-            if t.numel() != (_scales(n) if name.endswith("scales") else n):
-                raise TritonAdamWUnavailable(f"{name} has the wrong number of elements.")
-    return device, sizes
+    if len(tensors) != len(sizes):
+        raise TritonAdamWUnavailable("all tensor lists must have the same length.")
+    for t, n in zip(tensors, sizes):
+        if (t.dtype is not dtype or t.numel() != n or t.get_device() != device
+                or not t.is_contiguous()):
+            raise TritonAdamWUnavailable(
+                f"{name} must be contiguous {dtype} tensors of {n} elements on one CUDA device; "
+                f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return [t.data_ptr() for t in tensors]
+
+
+def _state_addresses(lists: Sequence[Sequence[Tensor]], sizes: Sequence[int], device: int):
+    scales = [(n + BLOCK - 1) // BLOCK for n in sizes]
+    return [_addresses(name, values, scales if name.endswith("scales") else sizes, dtype, device)
+            for values, (name, dtype) in zip(lists, _STATE.items())], scales
 
 
 def _per_tensor(value, count: int, name: str) -> list:
@@ -59,13 +59,15 @@ def _per_tensor(value, count: int, name: str) -> list:
     return [value] * count
 
 
-def _refuse_shared(name: str, tensors: Sequence[Tensor]) -> None:
+def _refuse_shared(name: str, addresses: Sequence[int], sizes: Sequence[int], width: int) -> None:
     """Two entries over the same memory would be updated by two blocks at once."""
 
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                   for t in tensors if t.numel())
-    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
-        raise TritonAdamWUnavailable(f"two of the {name} share memory.")
+    end = 0
+    for at, n in sorted(zip(addresses, sizes)):
+        if n:
+            if at < end:
+                raise TritonAdamWUnavailable(f"two of the {name} share memory.")
+            end = at + n * width
 
 
 @torch.no_grad()
@@ -87,35 +89,31 @@ def adamw8bit_step(params: Sequence[Tensor], grads: Sequence[Tensor],
     """
 
     count = len(params)
-    device, numels = _check_states(
-        (exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales),
-        [p.numel() for p in params])
-    if count != len(grads) or count != len(numels):
-        raise TritonAdamWUnavailable("all tensor lists must have the same length.")
-    if count == 0:
+    if count == 0 and not any(map(len, (grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes,
+                                        exp_avg_sq_scales))):
         return
-    ops.check_device(device, TritonAdamWUnavailable)
-    dtype = params[0].dtype
-    code = ops._dtype_code(params[0], TritonAdamWUnavailable)
+    if count == 0:
+        raise TritonAdamWUnavailable("all tensor lists must have the same length.")
+    first = params[0]
+    ops.check_device(first.device, TritonAdamWUnavailable)
+    code = ops._dtype_code(first, TritonAdamWUnavailable)
+    dtype, device = first.dtype, first.get_device()
+    sizes = [p.numel() for p in params]
+    at_params = _addresses("parameters", params, sizes, dtype, device)
+    at_grads = _addresses("gradients", grads, sizes, dtype, device)
     for p, g in zip(params, grads):
-        if p.dtype != dtype or g.dtype != dtype or p.device != device or g.device != device:
-            raise TritonAdamWUnavailable("parameters and gradients must share dtype and device.")
-        if p.shape != g.shape or not p.is_contiguous() or not g.is_contiguous():
-            raise TritonAdamWUnavailable(
-                "parameters and gradients must be contiguous and of the same shape.")
-    for name, values in (("parameters", params), ("exp_avg codes", exp_avg_codes),
-                         ("exp_avg scales", exp_avg_scales),
-                         ("exp_avg_sq codes", exp_avg_sq_codes),
-                         ("exp_avg_sq scales", exp_avg_sq_scales)):
-        _refuse_shared(name, values)
-    address = lambda values: [t.data_ptr() for t in values]  # noqa: E731
-    with ops._OnDevice(device):
-        _capi.adamw8_step(address(params), address(grads), address(exp_avg_codes),
-                          address(exp_avg_scales), address(exp_avg_sq_codes),
-                          address(exp_avg_sq_scales), numels, _per_tensor(step, count, "step"),
-                          _per_tensor(lr, count, "lr"),
+        if p.shape != g.shape:
+            raise TritonAdamWUnavailable("parameters and gradients must have the same shapes.")
+    at_states, scales = _state_addresses(
+        (exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales), sizes, device)
+    _refuse_shared("parameters", at_params, sizes, first.element_size())
+    for name, at, width in zip(_STATE, at_states, (1, 4, 1, 4)):
+        _refuse_shared(name, at, scales if width == 4 else sizes, width)
+    with ops._OnDevice(first.device):
+        _capi.adamw8_step(at_params, at_grads, *at_states, sizes,
+                          _per_tensor(step, count, "step"), _per_tensor(lr, count, "lr"),
                           _per_tensor(weight_decay, count, "weight_decay"), beta1, beta2, eps,
-                          maximize, code, ops._stream(device), TritonAdamWUnavailable)
+                          maximize, code, ops._stream(first.device), TritonAdamWUnavailable)
 
 
 @torch.no_grad()
@@ -123,25 +121,23 @@ def adamw8bit_moments(exp_avg_codes: Sequence[Tensor], exp_avg_scales: Sequence[
                       exp_avg_sq_codes: Sequence[Tensor],
                       exp_avg_sq_scales: Sequence[Tensor]) -> tuple[list[Tensor], list[Tensor]]:
     """The fp32 ``(exp_avg, exp_avg_sq)`` lists that 8-bit states stand for, shaped like their
-    codes: for inspection, or to carry on with an optimizer that keeps 32-bit states. The tensors
-    of one call share one allocation."""
+    codes: for inspection, or to carry on with an optimizer that keeps 32-bit states."""
 
     held = (exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales)
-    device, numels = _check_states(held, None)
-    if not numels:
+    if not any(map(len, held)):
         return [], []
+    if len(exp_avg_codes) == 0:
+        raise TritonAdamWUnavailable("all tensor lists must have the same length.")
+    device = exp_avg_codes[0].device
     ops.check_device(device, TritonAdamWUnavailable)
-    # 32-byte aligned pieces of one buffer.
-    room = [(n + 7) // 8 * 8 for n in numels]
-    buffer = torch.empty(2 * sum(room), dtype=torch.float32, device=device)
-    pieces = buffer.split(room + room)
-    moments = [t[:n].view(c.shape) for t, n, c in
-               zip(pieces, numels + numels, [*exp_avg_codes, *exp_avg_codes])]
-    exp_avg, exp_avg_sq = moments[:len(numels)], moments[len(numels):]
-    address = lambda values: [t.data_ptr() for t in values]  # noqa: E731
+    sizes = [c.numel() for c in exp_avg_codes]
+    at_states, _ = _state_addresses(held, sizes, exp_avg_codes[0].get_device())
+    exp_avg, exp_avg_sq = ([torch.empty(c.shape, dtype=torch.float32, device=device)
+                            for c in exp_avg_codes] for _ in range(2))
     with ops._OnDevice(device):
-        _capi.adamw8_moments(*(address(v) for v in held), numels, address(exp_avg),
-                             address(exp_avg_sq), ops._stream(device), TritonAdamWUnavailable)
+        _capi.adamw8_moments(*at_states, sizes, [t.data_ptr() for t in exp_avg],
+                             [t.data_ptr() for t in exp_avg_sq], ops._stream(device),
+                             TritonAdamWUnavailable)
     return exp_avg, exp_avg_sq
 
 

@@ -40,6 +40,8 @@ def _per_token(t: Tensor, targets: Tensor, name: str) -> Tensor:
     if t.shape != targets.shape:
         raise TritonLogitLossUnavailable(
             f"{name} must have the targets' shape {tuple(targets.shape)}, not {tuple(t.shape)}")
+    if t.dtype is torch.float32 and not t.requires_grad:
+        return t
     return t.detach().to(torch.float32)
 
 

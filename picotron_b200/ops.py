@@ -33,6 +33,8 @@ type for that op (``Triton*Unavailable``); there is no fallback path.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import Tensor
 
@@ -649,38 +651,73 @@ def _ce_backward(ctx, grad, _grad_lse, _grad_mean):
 cross_entropy.register_autograd(_ce_backward, setup_context=_ce_setup)
 
 
-# The ops below are registered through torch.library.Library with an autograd.Function each,
-# where those above use custom_op: the same torch.ops.picotron_b200 entries and fake
-# implementations, but a forward + backward call costs 42 us of host time instead of 148
-# (measured without kernels), which is what a small call takes.
+# The ops below are registered through torch.library.Library with an autograd.Function each, where
+# those above use custom_op: the same torch.ops.picotron_b200 entries, fake implementations and
+# autograd, but small calls take the host's time, and a forward and backward through custom_op
+# spent 148 us there, one through Library and Function 42 (without kernels). Calls on plain
+# tensors outside of tracing and dispatch modes skip the dispatcher as well.
 
 _LIBRARY = torch.library.Library("picotron_b200", "FRAGMENT")
+_PLAIN = (Tensor, torch.nn.Parameter)
 
 
-def _register(schema: str, run, fake, function: type[torch.autograd.Function] | None = None):
-    """Define an op with its implementation (which checks the device itself), its fake one and, for
-    a differentiable op, the autograd Function to take where the first argument that may need
-    a gradient does; returns the op."""
+def _is_eager(args) -> bool:
+    """Whether nothing but autograd wants to see the call."""
 
-    name = schema.split("(")[0]
-    _LIBRARY.define(schema)
-    _LIBRARY.impl(name, run, "CompositeExplicitAutograd")
-    torch.library.register_fake(f"picotron_b200::{name}", fake, lib=_LIBRARY)
-    op = getattr(torch.ops.picotron_b200, name).default
-    if function is not None:
-        def autograd(*args):
-            if torch.is_grad_enabled() and any(
-                    isinstance(a, Tensor) and a.requires_grad for a in args):
-                return function.apply(*args)
-            return _below_autograd(op, *args)
-
-        _LIBRARY.impl(name, autograd, "Autograd")
-    return op
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
+            or torch._C._are_functorch_transforms_active()):
+        return False
+    for a in args:
+        if isinstance(a, Tensor) and type(a) not in _PLAIN:
+            return False
+    return True
 
 
-def _below_autograd(op, *args):
-    with torch._C._AutoDispatchBelowAutograd():
-        return op(*args)
+class _Op:
+    """A torch.ops.picotron_b200 op with its implementation (which checks the device itself), its
+    fake one and, for a differentiable op, the autograd Function that calls it ``below``."""
+
+    def __init__(self, schema: str, run, fake,
+                 function: type[torch.autograd.Function] | None = None) -> None:
+        name = schema.split("(")[0]
+        _LIBRARY.define(schema)
+        _LIBRARY.impl(name, run, "CompositeExplicitAutograd")
+        torch.library.register_fake(f"picotron_b200::{name}", fake, lib=_LIBRARY)
+        self.run, self.function = run, function
+        self.op = getattr(torch.ops.picotron_b200, name).default
+        if function is not None:
+            _LIBRARY.impl(name, self._autograd, "Autograd")
+
+    def _autograd(self, *args):
+        if torch.is_grad_enabled():
+            for a in args:
+                if isinstance(a, Tensor) and a.requires_grad:
+                    return self.function.apply(*args)
+        return self.below(*args)
+
+    def below(self, *args):
+        if _is_eager(args[:1]):
+            return self.run(*args)
+        with torch._C._AutoDispatchBelowAutograd():
+            return self.op(*args)
+
+    def __call__(self, *args):
+        if not _is_eager(args):
+            return self.op(*args)
+        return self._autograd(*args) if self.function is not None else self.run(*args)
+
+
+def _first_order(backward):
+    """A Function's backward whose own derivative is refused. Only a backward that is itself
+    recorded (create_graph) pays for torch's check of that."""
+
+    refusing = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return call
 
 
 # ------------------------------------------------------ losses over log-probabilities --
@@ -710,6 +747,8 @@ def _ll_rows(t: Tensor) -> tuple[int, int, int]:
 def _ll_logits(logits: Tensor) -> Tensor:
     """Logits with a contiguous class dimension and rows that do not overlap, copied if needed."""
 
+    if logits.is_contiguous():
+        return logits
     if logits.stride(-1) != 1 and logits.size(-1) > 1:
         return logits.contiguous()
     reach = logits.size(-1)
@@ -746,10 +785,19 @@ def _ll_logits_rows(logits: Tensor) -> tuple[int, int, int]:
     return logits.data_ptr(), logits.stride(0), logits.stride(1)
 
 
+@functools.lru_cache(maxsize=256)
+def _ll_workspace_size(vocab: int, outer: int, inner: int, code: int, device: int | None) -> int:
+    return max(16, _capi.logit_loss_workspace(vocab, outer, inner, code,
+                                              TritonLogitLossUnavailable))
+
+
 def _ll_workspace(logits: Tensor, outer: int, inner: int) -> Tensor:
-    size = _capi.logit_loss_workspace(logits.size(-1), outer, inner, DTYPE_CODES[logits.dtype],
-                                      TritonLogitLossUnavailable)
-    return torch.empty(max(size, 16), dtype=torch.uint8, device=logits.device)
+    """The forward's workspace; called with the logits' device current (its SM count sets the
+    size)."""
+
+    size = _ll_workspace_size(logits.size(-1), outer, inner, DTYPE_CODES[logits.dtype],
+                              logits.device.index)
+    return torch.empty(size, dtype=torch.uint8, device=logits.device)
 
 
 def _ll_dense_gradient(logits: Tensor) -> bool:
@@ -768,11 +816,14 @@ def _ll_gradient(logits: Tensor) -> Tensor:
     strided view of odd-sized rows."""
 
     shift = logits.data_ptr() % 16 // logits.element_size()
-    if _ll_dense_gradient(logits):
-        strides, span = torch.empty(logits.shape, device="meta").stride(), logits.numel()
-    else:
-        strides = logits.stride()
-        span = 1 + sum((n - 1) * st for n, st in zip(logits.shape, strides))
+    dense = _ll_dense_gradient(logits)
+    if dense and shift == 0:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if dense:
+        buffer = torch.empty(logits.numel() + shift, dtype=logits.dtype, device=logits.device)
+        return buffer[shift:].view(logits.shape)
+    strides = logits.stride()
+    span = 1 + sum((n - 1) * st for n, st in zip(logits.shape, strides))
     buffer = torch.empty(span + shift, dtype=logits.dtype, device=logits.device)
     return buffer.as_strided(logits.shape, strides, shift)
 
@@ -802,21 +853,39 @@ def _logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: T
     """dlogits = coef * grad * (onehot(targets) - softmax(logits)); coef has the targets' shape
     (and any strides), grad is one value."""
 
-    x, outer, inner = _ll_inputs(logits, targets, (coef,))
+    _ll_inputs(logits, targets, (coef,))
     if stats.shape != (*targets.shape, 2) or not stats.is_contiguous():
         raise TritonLogitLossUnavailable("stats must be the forward's.")
+    return _ll_backward(logits, targets, stats, coef, grad, ignore_index)
+
+
+def _ll_backward(logits, targets, stats, coef, grad, ignore_index) -> Tensor:
+    """logit_loss_backward of tensors that a forward has checked."""
+
+    x = _ll_logits(logits)
+    outer, inner = (1, x.size(0)) if x.dim() == 2 else (x.size(0), x.size(1))
     dlogits = _ll_gradient(x)
-    if dlogits.numel() == 0:
+    if outer * inner == 0:
         return dlogits
     if grad is not None:
         grad = grad.to(torch.float32)
+    if coef.dtype is not torch.float32:
+        coef = coef.to(torch.float32)
     with _OnDevice(x.device):
         _capi.token_logps_bwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
-                              int(ignore_index), stats.data_ptr(), _ll_rows(coef),
+                              ignore_index, stats.data_ptr(), _ll_rows(coef),
                               grad.data_ptr() if grad is not None else None,
                               _ll_logits_rows(dlogits), DTYPE_CODES[x.dtype], _stream(x.device),
                               TritonLogitLossUnavailable)
     return dlogits
+
+
+def _ll_backward_of(ctx_tensors, grad, ignore_index) -> Tensor:
+    """The logits gradient in a Function's backward, from (logits, targets, stats, coef)."""
+
+    if _is_eager(ctx_tensors[:1]):
+        return _ll_backward(*ctx_tensors, grad, ignore_index)
+    return logit_loss_backward.op(*ctx_tensors, grad, ignore_index)
 
 
 def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
@@ -826,7 +895,7 @@ def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
     return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
 
 
-logit_loss_backward = _register(
+logit_loss_backward = _Op(
     "logit_loss_backward(Tensor logits, Tensor targets, Tensor stats, Tensor coef, Tensor? grad, "
     "int ignore_index) -> Tensor", _logit_loss_backward, _logit_loss_backward_fake)
 
@@ -834,7 +903,7 @@ logit_loss_backward = _register(
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index):
-        logps, stats = _below_autograd(token_logps, logits, targets, ignore_index)
+        logps, stats = token_logps.below(logits, targets, ignore_index)
         ctx.save_for_backward(logits, targets, stats)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(stats)
@@ -842,14 +911,15 @@ class _TokenLogps(torch.autograd.Function):
         return logps, stats
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, grad, _grad_stats):
         if grad is None:
             return None, None, None
-        return logit_loss_backward(*ctx.saved_tensors, grad, None, ctx.ignore_index), None, None
+        dlogits = _ll_backward_of((*ctx.saved_tensors, grad), None, ctx.ignore_index)
+        return dlogits, None, None
 
 
-token_logps = _register(
+token_logps = _Op(
     "token_logps(Tensor logits, Tensor targets, int ignore_index) -> (Tensor, Tensor)",
     _token_logps, _token_logps_fake, _TokenLogps)
 
@@ -886,7 +956,7 @@ def _preference_loss_fake(logits, targets, reference, beta, label_smoothing, ign
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, reference, beta, label_smoothing, ignore_index):
-        loss, *rest = _below_autograd(preference_loss, logits, targets, reference, beta,
+        loss, *rest = preference_loss.below(logits, targets, reference, beta,
                                       label_smoothing, ignore_index)
         rewards, stats, coef = rest
         ctx.save_for_backward(logits, targets, stats, coef)
@@ -896,18 +966,17 @@ class _PreferenceLoss(torch.autograd.Function):
         return loss, rewards, stats, coef
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, grad, *_):
         if grad is None:
             return (None,) * 6
         logits, targets, stats, coef = ctx.saved_tensors
-        dlogits = logit_loss_backward(logits, targets, stats,
-                                      coef[:, None].expand(targets.shape), grad,
-                                      ctx.ignore_index)
+        dlogits = _ll_backward_of((logits, targets, stats, coef[:, None].expand(targets.shape)),
+                                  grad, ctx.ignore_index)
         return dlogits, None, None, None, None, None
 
 
-preference_loss = _register(
+preference_loss = _Op(
     "preference_loss(Tensor logits, Tensor targets, Tensor reference, float beta, "
     "float label_smoothing, int ignore_index) -> (Tensor, Tensor, Tensor, Tensor)",
     _preference_loss, _preference_loss_fake, _PreferenceLoss)
@@ -980,16 +1049,19 @@ def _one_pass_policy(logits: Tensor, targets: Tensor, expected: float | None) ->
 
     if expected is None and logits.dtype != torch.float16:
         expected = 1.0
-    # A traced graph (its tensors are subclasses) cannot carry the in-place rescaling and takes
-    # the two passes.
-    if expected is None or type(logits) not in (Tensor, torch.nn.Parameter):
+    # A traced graph cannot carry the in-place rescaling and takes the two passes.
+    if expected is None or not _is_eager((logits,)):
         return None
     outer, inner = _ll_geometry(logits, targets)
     code = _dtype_code(logits, TritonLogitLossUnavailable)
-    if logits.size(-1) < 1 or not _capi.policy_loss_grad_supported(
-            logits.size(-1), outer, inner, code, TritonLogitLossUnavailable):
+    if logits.size(-1) < 1 or not _ll_one_pass(logits.size(-1), outer, inner, code):
         return None
     return expected
+
+
+@functools.lru_cache(maxsize=256)
+def _ll_one_pass(vocab: int, outer: int, inner: int, code: int) -> bool:
+    return _capi.policy_loss_grad_supported(vocab, outer, inner, code, TritonLogitLossUnavailable)
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -998,10 +1070,10 @@ class _PolicyLoss(torch.autograd.Function):
         *args, expected = args
         ctx.expected = _one_pass_policy(logits, targets, expected)
         if ctx.expected is None:
-            loss, *rest = _below_autograd(policy_loss, logits, targets, *args, expected)
+            loss, *rest = policy_loss.below(logits, targets, *args, expected)
             ctx.dlogits = None
         else:
-            loss, *rest, ctx.dlogits = _below_autograd(policy_loss_grad, logits, targets, *args,
+            loss, *rest, ctx.dlogits = policy_loss_grad.below(logits, targets, *args,
                                                        ctx.expected)
         logps, stats, coef = rest
         ctx.save_for_backward(logits, targets, stats, coef)
@@ -1011,14 +1083,14 @@ class _PolicyLoss(torch.autograd.Function):
         return loss, logps, stats, coef
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, grad, *_):
         if grad is None:
             return (None,) * 11
         logits, targets, stats, coef = ctx.saved_tensors
         dlogits, ctx.dlogits = ctx.dlogits, None
         if dlogits is None:  # two passes, or a second backward through a retained graph
-            dlogits = logit_loss_backward(logits, targets, stats, coef, grad, ctx.ignore_index)
+            dlogits = _ll_backward_of((logits, targets, stats, coef), grad, ctx.ignore_index)
         elif dlogits.numel():
             outer, inner = _ll_geometry(logits, targets)
             grad = grad.to(torch.float32)
@@ -1033,10 +1105,10 @@ class _PolicyLoss(torch.autograd.Function):
 _POLICY = ("(Tensor logits, Tensor targets, Tensor old_logps, Tensor advantages, "
            "Tensor? reference, float clip_low, float clip_high, float kl_coef, bool by_sequence, "
            "int ignore_index, ")
-policy_loss_grad = _register(
+policy_loss_grad = _Op(
     f"policy_loss_grad{_POLICY}float grad) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
     _policy_loss_grad, _policy_loss_grad_fake)
-policy_loss = _register(
+policy_loss = _Op(
     f"policy_loss{_POLICY}float? expected_grad) -> (Tensor, Tensor, Tensor, Tensor)",
     _policy_loss, _policy_loss_fake, _PolicyLoss)
 
@@ -1203,8 +1275,7 @@ def _rope_qk_bwd(ctx, dq: Tensor | None, dk: Tensor | None):
 rope_qk.register_autograd(_rope_qk_bwd, setup_context=_rope_qk_setup)
 
 
-def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tensor,
-                           inv_freq: Tensor, layout: int, scale: float) -> tuple[Tensor, Tensor]:
+def _rope_positions_check(q, k, positions, inv_freq, layout) -> None:
     check_device(q.device, TritonRoPEUnavailable)
     for t in (k, positions, inv_freq):
         if t.device != q.device:
@@ -1212,18 +1283,22 @@ def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tens
                                         "device.")
     if layout not in (_capi.PT_ROPE_INTERLEAVED, _capi.PT_ROPE_ROTATE_HALF):
         raise TritonRoPEUnavailable(f"unknown RoPE layout {layout}")
-    code = _dtype_code(q, TritonRoPEUnavailable)
-    if q.dim() != 4 or k.dim() != 4 or k.dtype != q.dtype or (
-            q.size(0), q.size(2), q.size(3)) != (k.size(0), k.size(2), k.size(3)):
+    _dtype_code(q, TritonRoPEUnavailable)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or k.dtype != q.dtype or (qs[0], qs[2], qs[3]) != (
+            ks[0], ks[2], ks[3]):
         raise TritonRoPEUnavailable("RoPE requires query and key [B, H, S, D] of one dtype that "
                                     "share B, S and D.")
-    if positions.dtype != torch.long or positions.shape not in ((q.size(2),),
-                                                                (q.size(0), q.size(2))):
+    if positions.dtype != torch.long or positions.shape not in ((qs[2],), (qs[0], qs[2])):
         raise TritonRoPEUnavailable("RoPE positions must be int64 [S] or [B, S].")
     if (inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.numel() < 1
-            or 2 * inv_freq.numel() > q.size(3)):
+            or 2 * inv_freq.numel() > qs[3]):
         raise TritonRoPEUnavailable("RoPE frequencies must be float64 [R/2] with R at most the "
                                     "head dimension.")
+
+
+def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tensor,
+                           inv_freq: Tensor, layout: int, scale: float) -> tuple[Tensor, Tensor]:
     q, q_out = _rope_state(q)
     k, k_out = _rope_state(k)
     if q.size(0) * q.size(2) == 0 or q.numel() + k.numel() == 0:
@@ -1234,7 +1309,7 @@ def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tens
         _capi.rope_positions(q.data_ptr(), q.stride(), q_out.data_ptr(), q_out.stride(), q.shape,
                              k.data_ptr(), k.stride(), k_out.data_ptr(), k_out.stride(), k.shape,
                              positions.data_ptr(), strides, inv_freq.data_ptr(),
-                             2 * inv_freq.numel(), scale, backward, layout, code,
+                             2 * inv_freq.numel(), scale, backward, layout, DTYPE_CODES[q.dtype],
                              _stream(q.device), TritonRoPEUnavailable)
     return q_out, k_out
 
@@ -1250,10 +1325,12 @@ def _rope_state(x: Tensor) -> tuple[Tensor, Tensor]:
 
 
 def _rope_positions(q, k, positions, inv_freq, layout, scale):
+    _rope_positions_check(q, k, positions, inv_freq, layout)
     return _rope_positions_launch(False, q, k, positions, inv_freq, layout, scale)
 
 
 def _rope_positions_backward(dq, dk, positions, inv_freq, layout, scale):
+    _rope_positions_check(dq, dk, positions, inv_freq, layout)
     return _rope_positions_launch(True, dq, dk, positions, inv_freq, layout, scale)
 
 
@@ -1266,22 +1343,26 @@ class _RopePositions(torch.autograd.Function):
     def forward(ctx, q, k, positions, inv_freq, layout, scale):
         ctx.save_for_backward(positions, inv_freq)
         ctx.layout, ctx.scale = layout, scale
-        ctx.metas = [(t.shape, t.dtype, t.device) for t in (q, k)]
+        ctx.metas = ((q.shape, q.dtype, q.device), (k.shape, k.dtype, k.device))
         ctx.set_materialize_grads(False)
-        return _below_autograd(rope_positions, q, k, positions, inv_freq, layout, scale)
+        return rope_positions.below(q, k, positions, inv_freq, layout, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, *grads):
-        grads = [torch.zeros(shape, dtype=dtype, device=device) if g is None else g
-                 for g, (shape, dtype, device) in zip(grads, ctx.metas)]
-        return (*rope_positions_backward(*grads, *ctx.saved_tensors, ctx.layout, ctx.scale),
-                None, None, None, None)
+        dq, dk = (torch.zeros(shape, dtype=dtype, device=device) if g is None else g
+                  for g, (shape, dtype, device) in zip(grads, ctx.metas))
+        args = (dq, dk, *ctx.saved_tensors, ctx.layout, ctx.scale)
+        if _is_eager((dq,)):
+            dq, dk = _rope_positions_launch(True, *args)
+        else:
+            dq, dk = rope_positions_backward.op(*args)
+        return dq, dk, None, None, None, None
 
 
 _ROPE_POSITIONS = ("(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, int layout, "
                    "float scale) -> (Tensor, Tensor)")
-rope_positions_backward = _register("rope_positions_backward" + _ROPE_POSITIONS,
-                                    _rope_positions_backward, _rope_positions_fake)
-rope_positions = _register("rope_positions" + _ROPE_POSITIONS, _rope_positions,
-                           _rope_positions_fake, _RopePositions)
+rope_positions_backward = _Op("rope_positions_backward" + _ROPE_POSITIONS,
+                              _rope_positions_backward, _rope_positions_fake)
+rope_positions = _Op("rope_positions" + _ROPE_POSITIONS, _rope_positions, _rope_positions_fake,
+                     _RopePositions)

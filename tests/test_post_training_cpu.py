@@ -74,7 +74,7 @@ def test_policy_gradient_support_and_rescaling_are_checked_before_cuda():
         lib.pt_policy_loss_grad_supported(vocab, outer, 1, dtype, ctypes.byref(flag)), flag.value)
     assert ask(128256) == (_capi.PT_OK, 1) and ask(786432) == (_capi.PT_OK, 1)
     assert ask(786433) == (_capi.PT_OK, 0) and ask(400_000, dtype=0) == (_capi.PT_OK, 0)
-    assert ask(8, 2**29) == (_capi.PT_OK, 0)
+    assert ask(8, 2**29) == (_capi.PT_OK, 0) and ask(8, 2**31)[0] == _capi.PT_ERR_SHAPE
     assert ask(0)[0] == _capi.PT_ERR_SHAPE and ask(8, dtype=4)[0] == _capi.PT_ERR_UNSUPPORTED_DTYPE
     rescale = lambda expected, dtype=2, outer=1: lib.pt_rescale_logits_grad(  # noqa: E731
         None, 8, outer, 1, 8, 8, None, expected, dtype, None)
