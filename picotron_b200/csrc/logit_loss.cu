@@ -2,14 +2,14 @@
 // (forward and backward), the preference loss of chosen / rejected pairs and the clipped policy
 // loss with a KL term, each with the gradient of its logits.
 //
-// For a row x with target t, relative to a reference m near max(x):
+// For a row x with target t, relative to a reference m a little above max(x):
 //   s = sum 2^((x - m) log2 e),  log softmax(x)_t = (x_t - m) - ln s.
 // x is taken relative to m before it is scaled, so a row of one type's lowest values (a mask
 // that leaves nothing) neither overflows nor loses its s. Losses sum these over thousands of
-// positions, where a bias matters more than a rounding: log2 e is applied in two parts, the mean
-// error of the exponential unit is taken out of each term, and sums are rescaled only when the
-// reference has fallen e^8 behind and once more when threads are merged. The differences are
-// taken in 64 bits and the log-probability is rounded once. Every loss here depends on the
+// positions, where a bias matters more than a rounding: log2 e is applied in two parts, sums are
+// rescaled only when a value passes the reference and once more when threads are merged, and
+// the mean error of the exponential unit is taken out of ln s. The differences are taken in 64
+// bits and the log-probability is rounded once. Every loss here depends on the
 // logits through these log-probabilities alone, so its gradient is
 //   dx = c (onehot(t) - softmax(x)),  softmax(x) = 2^((x - m) log2 e) / s,
 // with one coefficient c per row: the forward keeps (m, 1/s) and c, the backward reads the
@@ -42,10 +42,13 @@ constexpr int kGradTrips = 4;
 constexpr int kSumThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f;  // log2(e): exp(a) = 2^(a log2(e))
 constexpr float kLog2eLow = (float)(1.4426950408889634 - (double)kLog2e);  // what it lacks
-// How far ex2.approx is below the true value on average (measured over 4 M points of [-20, 0] on
-// B200; its largest error is 1.4e-7).
+// How far ex2.approx is below the true value on average for arguments below 0 (measured over 10^6
+// points of [-20, 0] on B200; its largest error there is 1.4e-7). Above 0 it is 3.3e-8 too high,
+// so the reference is kept above every value: by kAbove when it is set, which leaves room for
+// larger values to come. References are whole numbers, so that most threads of a row have the
+// same one and their sums merge without a factor.
 constexpr float kExpLow = 5.05e-8f;
-constexpr float kRaise = 8.0f;  // how far a value may pass the reference: e^8 V stays in range
+constexpr float kAbove = 8.0f;
 constexpr int kErrBadTarget = 2;
 
 // Row r of the [outer, inner] row grid sits at outer index r / inner, inner index r % inner. One
@@ -90,13 +93,28 @@ __device__ __forceinline__ float2 log2_scaled(float2 d) {  // d log2(e)
   return __ffma2_rn(d, splat2(kLog2e), __fmul2_rn(d, splat2(kLog2eLow)));
 }
 __device__ __forceinline__ float fast_exp(float d) {
-  const float y = fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
-  return fmaf(y, kExpLow, y);
+  return fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+}
+// e^-k, rounded once, for the whole numbers that references differ by.
+constexpr int kWholePowers = 32;
+struct WholePowers {
+  float p[kWholePowers];
+  constexpr WholePowers() : p() {
+    double v = 1.0;
+    for (int k = 0; k < kWholePowers; ++k, v *= 0.36787944117144233) p[k] = (float)v;
+  }
+};
+__constant__ WholePowers c_powers{};
+__device__ __noinline__ float exact_exp(float d) { return (float)exp((double)d); }
+// e^-d for two references that are d >= 0 apart.
+__device__ __forceinline__ float factor_below(float d) {
+  if (d < (float)kWholePowers) return c_powers.p[(int)d];
+  return exact_exp(-d);
 }
 
 // The sum of v relative to the reference m >= v.m. A NaN sum stays NaN (NaN * 0).
 __device__ __forceinline__ float sum_at(Stat v, float m) {
-  return v.m == m ? v.s : v.s * (v.m == -INFINITY ? 0.0f : fast_exp(v.m - m));
+  return v.m == m ? v.s : v.s * (v.m == -INFINITY ? 0.0f : factor_below(m - v.m));
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -124,9 +142,10 @@ struct Running {
   float m = -INFINITY;
   float2 s = make_float2(0.0f, 0.0f);
   __device__ __forceinline__ void raise(float xmax) {
-    if (xmax > m + kRaise || m == -INFINITY) {
-      s = __fmul2_rn(s, splat2(m == -INFINITY ? 0.0f : fast_exp(m - xmax)));
-      m = xmax;
+    if (xmax > m) {
+      const float above = ceilf(xmax) + kAbove;
+      s = __fmul2_rn(s, splat2(m == -INFINITY ? 0.0f : factor_below(above - m)));
+      m = above;
     }
   }
   // What x is taken relative to. Only -inf (which add 0) or NaN so far: 0 gives those results.
@@ -146,14 +165,9 @@ struct Running {
   }
   __device__ __forceinline__ void add1(float x) {
     raise(x);
-    const float d = x - base();
-    s.x += fast_exp2(fmaf(d, kLog2e, d * kLog2eLow));
+    s.x += fast_exp(x - base());
   }
-  // With the exponentials' mean error taken out, of all but the reference's own, which is 1.
-  __device__ __forceinline__ Stat stat() const {
-    const float sum = s.x + s.y;
-    return {m, m == -INFINITY ? sum : fmaf(sum - 1.0f, kExpLow, sum)};
-  }
+  __device__ __forceinline__ Stat stat() const { return {m, s.x + s.y}; }
 };
 
 // log softmax at the value xt. The differences are taken first: m may be as large as the type
@@ -165,8 +179,10 @@ __device__ __forceinline__ double log_softmax(Stat v, float xt) {
   const int k = bits >> 23;
   const float f = __int_as_float((bits & 0x007fffff) + 0x3f3504f3);
   // s - s is 0, or NaN where s is not finite and has no such k and f.
-  return ((double)xt - (double)v.m) -
-         ((double)k * 0.6931471805599453 + (double)(logf(f) + (v.s - v.s)));
+  const double lp = ((double)xt - (double)v.m) -
+                    ((double)k * 0.6931471805599453 + (double)kExpLow) -
+                    (double)(logf(f) + (v.s - v.s));
+  return lp > 0.0 ? 0.0 : lp;  // a near-certain target is within rounding of 0 on either side
 }
 
 // Elements before the first 16-byte boundary of a row (0 when it is aligned).
@@ -688,15 +704,13 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
   __syncwarp();
   if (w1 > w0 && !mbar_wait_bounded(&bar[warp], 0) && lane == 0)
     atomicExch(&g_logit_loss_error, kErrWait);
-  // Two vectors a trip, each with its own sums: twice the independent additions.
-  Running acc2;
+  // Two vectors a trip: their loads and exponentials overlap.
   int v = w0 + lane;
   for (; v + 32 < w1; v += 64) {
-    float x[V], y[V];
+    float x[2 * V];
     unpack<T>(lds128(slice + (size_t)v * 16), x);
-    unpack<T>(lds128(slice + (size_t)(v + 32) * 16), y);
-    acc.template add<V>(x);
-    acc2.template add<V>(y);
+    unpack<T>(lds128(slice + (size_t)(v + 32) * 16), x + V);
+    acc.template add<2 * V>(x);
   }
   if (v < w1) {
     float x[V];
@@ -707,9 +721,7 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
-  const Stat s1 = acc.stat(), s2 = acc2.stat();
-  const float both = fmaxf(s1.m, s2.m);
-  Stat total = block_merge(Stat{both, sum_at(s1, both) + sum_at(s2, both)}, red);
+  Stat total = block_merge(acc.stat(), red);
   if (cluster > 1 && tid < cluster) store_in_cluster(&peer[rank], &peer_bar, tid, total);
   if (tid == 0) {
     if (cluster > 1) {

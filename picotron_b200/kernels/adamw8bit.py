@@ -113,7 +113,9 @@ def adamw8bit_step(params: Sequence[Tensor], grads: Sequence[Tensor],
         _capi.adamw8_step(at_params, at_grads, *at_states, sizes,
                           _per_tensor(step, count, "step"), _per_tensor(lr, count, "lr"),
                           _per_tensor(weight_decay, count, "weight_decay"), beta1, beta2, eps,
-                          maximize, code, ops._stream(first.device), TritonAdamWUnavailable)
+                          maximize, code, ops._raw_stream(first.device), TritonAdamWUnavailable)
+    # As an in-place torch operation does: a backward that saved a parameter notices.
+    torch.autograd.graph.increment_version(params)
 
 
 @torch.no_grad()
@@ -136,7 +138,7 @@ def adamw8bit_moments(exp_avg_codes: Sequence[Tensor], exp_avg_scales: Sequence[
                             for c in exp_avg_codes] for _ in range(2))
     with ops._OnDevice(device):
         _capi.adamw8_moments(*at_states, sizes, [t.data_ptr() for t in exp_avg],
-                             [t.data_ptr() for t in exp_avg_sq], ops._stream(device),
+                             [t.data_ptr() for t in exp_avg_sq], ops._raw_stream(device),
                              TritonAdamWUnavailable)
     return exp_avg, exp_avg_sq
 
@@ -186,7 +188,8 @@ class AdamW8bit(Optimizer):
                 calls[(p.device, p.dtype, *key)].append((p, group))
         for (_, _, beta1, beta2, eps, maximize), items in calls.items():
             params = [p for p, _ in items]
-            states = [self.state[p] if self.state[p] else self._new_state(p) for p in params]
+            # Not self.state[p], which would leave an empty entry behind a refused step.
+            states = [self.state.get(p) or self._new_state(p) for p in params]
             adamw8bit_step(params, [p.grad for p in params],
                            *([s[name] for s in states] for name in _STATE),
                            step=[s["step"] + 1 for s in states],

@@ -92,6 +92,12 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _raw_stream(device: torch.device) -> int:
+    """_stream without the Stream object (0.1 against 2.3 us of host time)."""
+
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 class _OnDevice:
     """Make ``device`` current for the duration of a C-ABI call (no-op when it is)."""
 
@@ -818,7 +824,7 @@ def _ll_gradient(logits: Tensor) -> Tensor:
     shift = logits.data_ptr() % 16 // logits.element_size()
     dense = _ll_dense_gradient(logits)
     if dense and shift == 0:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return torch.empty_like(logits, memory_format=torch.contiguous_format)
     if dense:
         buffer = torch.empty(logits.numel() + shift, dtype=logits.dtype, device=logits.device)
         return buffer[shift:].view(logits.shape)
@@ -839,7 +845,7 @@ def _token_logps(logits: Tensor, targets: Tensor, ignore_index: int) -> tuple[Te
         _capi.token_logps_fwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
                               int(ignore_index), logps.data_ptr(), stats.data_ptr(),
                               work.data_ptr(), work.numel(), DTYPE_CODES[x.dtype],
-                              _stream(x.device), TritonLogitLossUnavailable)
+                              _raw_stream(x.device), TritonLogitLossUnavailable)
     return logps, stats
 
 
@@ -875,7 +881,7 @@ def _ll_backward(logits, targets, stats, coef, grad, ignore_index) -> Tensor:
         _capi.token_logps_bwd(_ll_logits_rows(x), x.size(-1), outer, inner, _ll_rows(targets),
                               ignore_index, stats.data_ptr(), _ll_rows(coef),
                               grad.data_ptr() if grad is not None else None,
-                              _ll_logits_rows(dlogits), DTYPE_CODES[x.dtype], _stream(x.device),
+                              _ll_logits_rows(dlogits), DTYPE_CODES[x.dtype], _raw_stream(x.device),
                               TritonLogitLossUnavailable)
     return dlogits
 
@@ -944,7 +950,7 @@ def _preference_loss(logits: Tensor, targets: Tensor, reference: Tensor, beta: f
                                   float(beta), float(label_smoothing), loss.data_ptr(),
                                   rewards.data_ptr(), stats.data_ptr(), coef.data_ptr(),
                                   work.data_ptr(), work.numel(), DTYPE_CODES[x.dtype],
-                                  _stream(x.device), TritonLogitLossUnavailable)
+                                  _raw_stream(x.device), TritonLogitLossUnavailable)
     return loss, rewards, stats, coef
 
 
@@ -1002,7 +1008,7 @@ def _policy_loss(logits: Tensor, targets: Tensor, old_logps: Tensor, advantages:
                               float(clip_low), float(clip_high), float(kl_coef),
                               by_sequence, loss.data_ptr(), logps.data_ptr(), stats.data_ptr(),
                               coef.data_ptr(), work.data_ptr(), work.numel(),
-                              DTYPE_CODES[x.dtype], _stream(x.device),
+                              DTYPE_CODES[x.dtype], _raw_stream(x.device),
                               TritonLogitLossUnavailable)
     return loss, logps, stats, coef
 
@@ -1032,7 +1038,7 @@ def _policy_loss_grad(logits, targets, old_logps, advantages, reference, clip_lo
                                clip_low, clip_high, kl_coef, by_sequence, grad, loss.data_ptr(),
                                logps.data_ptr(), stats.data_ptr(), coef.data_ptr(),
                                _ll_logits_rows(dlogits), work.data_ptr(), work.numel(),
-                               DTYPE_CODES[x.dtype], _stream(x.device),
+                               DTYPE_CODES[x.dtype], _raw_stream(x.device),
                                TritonLogitLossUnavailable)
     return loss, logps, stats, coef, dlogits
 
@@ -1097,7 +1103,7 @@ class _PolicyLoss(torch.autograd.Function):
             with _OnDevice(logits.device):
                 _capi.rescale_logits_grad(_ll_logits_rows(dlogits), dlogits.size(-1), outer,
                                           inner, grad.data_ptr(), ctx.expected,
-                                          DTYPE_CODES[logits.dtype], _stream(logits.device),
+                                          DTYPE_CODES[logits.dtype], _raw_stream(logits.device),
                                           TritonLogitLossUnavailable)
         return dlogits, *(None,) * 10
 
@@ -1310,7 +1316,7 @@ def _rope_positions_launch(backward: bool, q: Tensor, k: Tensor, positions: Tens
                              k.data_ptr(), k.stride(), k_out.data_ptr(), k_out.stride(), k.shape,
                              positions.data_ptr(), strides, inv_freq.data_ptr(),
                              2 * inv_freq.numel(), scale, backward, layout, DTYPE_CODES[q.dtype],
-                             _stream(q.device), TritonRoPEUnavailable)
+                             _raw_stream(q.device), TritonRoPEUnavailable)
     return q_out, k_out
 
 

@@ -278,6 +278,36 @@ def test_training_loop_step_object_runs_it():
     assert all(opt.state[p]["step"] == 1 for p in ps)
 
 
+def test_parameters_notice_the_step():
+    """A graph that saved a parameter before the step refuses to go back through it after."""
+
+    p = torch.nn.Parameter(gu.randn((8, 8), 5))
+    p.grad = gu.randn((8, 8), 6)
+    x = gu.randn((8, 8), 7).requires_grad_()
+    out = (x @ p).sum()
+    AdamW8bit([p]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
+def test_captured_step_and_refused_step():
+    p, g, state = _fresh(5000, torch.bfloat16, 12)
+    q, s2 = p.clone(), [t.clone() for t in state]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _call([q], [g], [s2], 1)
+    for _ in range(2):  # a graph repeats the step that it captured, with its step count
+        graph.replay()
+        _call([p], [g], [state], 1)
+    assert torch.equal(p, q) and all(torch.equal(a, b) for a, b in zip(state, s2))
+    bad = torch.nn.Parameter(gu.randn((6, 4), 1).t())
+    bad.grad = torch.zeros_like(bad)
+    opt = AdamW8bit([bad])
+    with pytest.raises(TritonAdamWUnavailable):
+        opt.step()
+    assert opt.moments() == {} and len(opt.state) == 0
+
+
 def test_streams_give_the_same_bits():
     p, g, state = _fresh(100_000, torch.float32, 9)
     q, s2 = p.clone(), [t.clone() for t in state]

@@ -9,7 +9,10 @@ Tolerances, for a row of V logits (u = 2^-24, the half step of fp32):
   of its own rounding;
 * a softmax value is one more such term over s: at most 2 EPS; dx = c (onehot - p) then has an
   absolute error of |c| p 2 EPS + |dc| + |dx| (4 u + half a step of the logits' type), and, where
-  the type's smallest step is coarser than that, half of it.
+  the type's smallest step is coarser than that, half of it;
+* the exponential's results below 2^-126 are 0. They are taken relative to a reference that is at
+  most 9 above the row's maximum, so s >= e^-9 (1 - EPS) and a softmax value below
+  2^-126 e^9 < 2^-113 may be 0 instead: another |c| 2^-113.
 dc is the error that the coefficient takes from the log-probabilities, derived per loss below.
 """
 
@@ -85,7 +88,7 @@ def _check_grad(got, x, t, coef, dcoef=0.0):
     dc = torch.as_tensor(dcoef, dtype=torch.float64)
     dc = dc.unsqueeze(-1) if dc.dim() else dc
     info = torch.finfo(x.dtype)
-    tol = c * p * 2 * _eps(x.size(-1)) + dc + want.abs() * (4 * U + info.eps / 2)
+    tol = c * (p * 2 * _eps(x.size(-1)) + 2.0 ** -113) + dc + want.abs() * (4 * U + info.eps / 2)
     tol = tol + info.smallest_normal * info.eps / 2
     err = (got.double().cpu() - want).abs()
     assert (err <= tol).all(), f"{(err - tol).max()} over at {want.abs().max()}"
@@ -169,6 +172,25 @@ def test_masked_logits(dtype):
     clean = x.detach().clone()
     clean[1, :3] = 0.0
     _check_grad(dx, clean, t, dlp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_near_certain_targets_and_large_logits(dtype):
+    """Targets far above the rest (log-probabilities next to 0, never above), and logits of any
+    size that the type holds."""
+
+    x, t = _data((4, 8, 515), dtype, seed=10, ignore=False)
+    top = torch.finfo(dtype).max
+    x[0].scatter_(-1, t[0, :, None], 40.0)
+    x[1] = (x[1].double() * 1000).to(dtype)
+    x[2] = torch.where(x[2] > 0, x[2].abs() + top / 4, x[2]).to(dtype)
+    x[3] += -top / 2
+    x.requires_grad_()
+    lp = kernels.token_log_probs(x, t)
+    assert (lp <= 0).all() and (lp[0] > -1e-6).all()
+    _check_logps(lp.detach(), x.detach(), t)
+    (dx,) = torch.autograd.grad(lp, x, torch.ones_like(lp))
+    _check_grad(dx, x.detach(), t, torch.ones(t.shape))
 
 
 def test_rows_without_a_finite_logit_are_nan():
