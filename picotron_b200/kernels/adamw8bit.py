@@ -218,6 +218,9 @@ class AdamW8bit(Optimizer):
         """torch's, with codes and scales kept in their own dtypes (the base class would cast
         them to the parameters')."""
 
+        for held in state_dict["state"].values():
+            if not {"step", *_STATE} <= held.keys():
+                raise ValueError("the state is not an AdamW8bit's: it lacks codes or scales")
         super().load_state_dict(state_dict)
         for saved, group in zip(state_dict["param_groups"], self.param_groups):
             for index, p in zip(saved["params"], group["params"]):

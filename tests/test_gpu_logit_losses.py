@@ -469,6 +469,57 @@ def test_policy_of_views(view):
         _check_policy(x, t, old, adv, ref, 0.1, "token", scales=(None,))
 
 
+@pytest.mark.parametrize("vocab", [65, 512])
+def test_gradients_through_a_slice_and_saved_on_the_host(vocab):
+    """The whole logits' gradient where the losses read a slice of them, and the same bits with
+    saved tensors kept in host memory (where strided views come back contiguous)."""
+
+    x, t = _data((4, 7, vocab), torch.bfloat16, seed=49)
+    old, ref, adv = (v[:, 1:] for v in _policy_inputs(x, t, 50))
+    leaf = x.detach().requires_grad_()
+    results = []
+    for hooks in (None, torch.autograd.graph.save_on_cpu()):
+        if hooks:
+            hooks.__enter__()
+        cut, want = leaf[:, :-1], t[:, 1:]
+        lp = kernels.token_log_probs(cut, want)
+        pref, _ = kernels.preference_loss(cut, want, ref)
+        pol, _ = kernels.policy_loss(cut, want, old, adv, reference_log_probs=ref, kl_coef=0.1)
+        if hooks:
+            hooks.__exit__(None, None, None)
+        results.append([torch.autograd.grad(v, leaf, u, retain_graph=True)[0]
+                        for v, u in ((lp, adv), (pref, None), (pol, None), (pol, None))])
+    for got in results:
+        for a, b in zip(got, results[0]):
+            assert torch.equal(a, b) and (a[:, -1] == 0).all()
+    _check_grad(results[0][0][:, :-1], x[:, :-1], t[:, 1:], adv)
+
+
+def test_empty_batches_have_empty_gradients():
+    x, t = _data((2, 3, 64), torch.bfloat16, seed=52)
+    f = torch.zeros(t.shape, device=gu.DEV)
+    for cut in ((slice(0, 0), slice(None)), (slice(None), slice(0, 0))):
+        leaf = x[cut].detach().requires_grad_()
+        loss, _ = kernels.policy_loss(leaf, t[cut], f[cut], f[cut])
+        (dx,) = torch.autograd.grad(loss, leaf)
+        assert math.isnan(loss.item()) and dx.shape == leaf.shape
+        loss, _ = kernels.preference_loss(leaf, t[cut], f[cut])
+        (dx,) = torch.autograd.grad(loss, leaf)
+        assert dx.shape == leaf.shape
+        lp = kernels.token_log_probs(leaf, t[cut])
+        (dx,) = torch.autograd.grad(lp.sum(), leaf)
+        assert dx.shape == leaf.shape
+
+
+def test_second_derivatives_are_refused():
+    x, t = _data((2, 3, 64), torch.float32, seed=53, ignore=False)
+    x.requires_grad_()
+    lp = kernels.token_log_probs(x, t)
+    (dx,) = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad((dx * dx).sum(), x)
+
+
 def test_compiled_graphs_agree():
     x, t = _data((2, 6, 501), torch.bfloat16, seed=47)
     old, ref, adv = _policy_inputs(x, t, 48)

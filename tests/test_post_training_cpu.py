@@ -234,6 +234,11 @@ def test_adamw8bit_state_dict_keeps_codes_and_scales(dtype):
         if name != "step":
             got = other.state[q][name]
             assert got.dtype == t.dtype and torch.equal(got, t) and got is not t
+    foreign = torch.optim.AdamW([q])
+    foreign.state[q] = {"step": torch.tensor(1.0), "exp_avg": torch.zeros(300),
+                        "exp_avg_sq": torch.zeros(300)}
+    with pytest.raises(ValueError, match="not an AdamW8bit"):
+        AdamW8bit([q]).load_state_dict(foreign.state_dict())
     for bad in (dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0), dict(betas=(1.0, 0.9)),
                 dict(betas=(0.9, -0.1))):
         with pytest.raises(ValueError):
