@@ -293,6 +293,61 @@ stats_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows,
   }
 }
 
+// Short rows: one warp per row, without the CTA's meetings. The policy loss holds a row in
+// registers: kShortVecs 16-byte vectors (8 KB) at most.
+constexpr int kShortVecs = 512;
+constexpr int kShortWarps = 4;  // rows per CTA
+
+// The element of an unaligned row's head (lanes below 16) or tail (the others) that a lane takes,
+// or -1; there are at most 7 of each.
+__device__ __forceinline__ int64_t edge_of(int lane, int head, int64_t tail, int64_t vocab) {
+  if (lane < head) return lane;
+  return lane >= 16 && tail + lane - 16 < vocab ? tail + lane - 16 : -1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kShortWarps * 32)
+stats_short_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows,
+                   int64_t vocab, RowOut out) {
+  constexpr int V = Vec16<T>::N;
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const RowIndex index = tg.index(r);
+  const int64_t t = tg.at(index);
+  const RowKind kind = row_kind(t, tg.ignore, vocab);
+  if (kind != kRowUsed) {
+    if (lane == 0) out.store(r, kind, Stat{0.0f, 1.0f}, 0.0f);
+    return;
+  }
+  const T* row = logits + lg.offset(index);
+  const float xt = to_float(row[t]);
+  const int head = head_elems(row, vocab);
+  const T* body = row + head;
+  const int nvec = (int)((vocab - head) / V);
+  const int64_t edge = edge_of(lane, head, head + (int64_t)nvec * V, vocab);
+  Running acc;
+  if (edge >= 0) acc.add1(to_float(row[edge]));
+  for (int v0 = lane; v0 < nvec; v0 += 32 * kUnrollStats) {
+    uint4 raw[kUnrollStats];
+#pragma unroll
+    for (int u = 0; u < kUnrollStats; ++u)
+      if (v0 + 32 * u < nvec) raw[u] = ld_stream(body + (v0 + 32 * u) * V);
+#pragma unroll
+    for (int u = 0; u < kUnrollStats; ++u) {
+      if (v0 + 32 * u < nvec) {
+        float x[V];
+        unpack<T>(raw[u], x);
+        acc.template add<V>(x);
+      }
+    }
+  }
+  const Stat v = acc.stat();
+  const float m = warp_max(v.m);
+  const float sum = warp_sum(sum_at(v, m));
+  if (lane == 0) out.store(r, kind, Stat{m, sum}, xt);
+}
+
 // Merges the splits of each row, one warp per row in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -315,6 +370,79 @@ finish_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows
       v.s = warp_sum(v.s);
     }
     if (lane == 0) out.store(r, kind, v, xt);
+  }
+}
+
+// How dx of one row is formed: dx = a e^(x - m), a = -c / s, and c more at the target.
+struct RowGrad {
+  float a, c, nm;
+  // V elements; the target, if it is among them, without its c.
+  template <typename T> __device__ __forceinline__ uint4 vec(const uint4& raw) const {
+    constexpr int V = Vec16<T>::N;
+    const float2 nm2 = splat2(nm), a2 = splat2(a), L = splat2(kLog2e);
+    float x[V];
+    unpack<T>(raw, x);
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2), L);
+      const float2 d = __fmul2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), a2);
+      x[e] = d.x;
+      x[e + 1] = d.y;
+    }
+    return pack<T>(x);
+  }
+  __device__ __forceinline__ float one(float x, bool target) const {
+    const float e = fast_exp(x + nm);
+    return target ? fmaf(a, e, c) : a * e;
+  }
+};
+
+// dx = c (onehot - softmax) of short rows, one warp per row.
+template <typename T>
+__global__ void __launch_bounds__(kShortWarps * 32)
+grad_short_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows,
+                  int64_t vocab, const float2* __restrict__ stats,
+                  const float* __restrict__ coef, RowGrid cg, const float* __restrict__ grad,
+                  T* __restrict__ dlogits, RowGrid dg) {
+  constexpr int V = Vec16<T>::N;
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const RowIndex index = tg.index(r);
+  const int64_t t = tg.at(index);
+  const bool used = row_kind(t, tg.ignore, vocab) == kRowUsed;
+  const T* row = logits + lg.offset(index);
+  T* drow = dlogits + dg.offset(index);
+  const int head = head_elems(row, vocab);
+  const int nvec = (int)((vocab - head) / V);
+  const int64_t edge = edge_of(lane, head, head + (int64_t)nvec * V, vocab);
+  const T* body = row + head;
+  T* dbody = drow + head;
+  if (!used) {
+    if (edge >= 0) drow[edge] = from_float<T>(0.0f);
+    for (int v = lane; v < nvec; v += 32) st_stream(dbody + v * V, make_uint4(0, 0, 0, 0));
+    return;
+  }
+  const float2 st = stats[r];
+  RowGrad f;
+  f.c = coef[cg.offset(index)] * (grad != nullptr ? *grad : 1.0f);
+  f.a = -f.c * st.y;
+  f.nm = -st.x;
+  if (edge >= 0) drow[edge] = from_float<T>(f.one(to_float(row[edge]), edge == t));
+  const int tv = t >= head && t < head + (int64_t)nvec * V ? (int)((t - head) / V) : -1;
+  for (int v0 = lane; v0 < nvec; v0 += 32 * kUnrollGrad) {
+    uint4 raw[kUnrollGrad];
+#pragma unroll
+    for (int u = 0; u < kUnrollGrad; ++u)
+      if (v0 + 32 * u < nvec) raw[u] = ld_stream(body + (v0 + 32 * u) * V);
+#pragma unroll
+    for (int u = 0; u < kUnrollGrad; ++u) {
+      const int v = v0 + 32 * u;
+      if (v < nvec) {
+        st_stream(dbody + v * V, f.vec<T>(raw[u]));
+        if (v == tv) drow[t] = from_float<T>(f.one(to_float(row[t]), true));
+      }
+    }
   }
 }
 
@@ -356,30 +484,15 @@ grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows, 
       continue;
     }
     const float2 st = stats[r];
-    const float c = coef[cg.offset(index)] * scale;
-    const float a = -c * st.y, nm = -st.x;
+    RowGrad f;
+    f.c = coef[cg.offset(index)] * scale;
+    f.a = -f.c * st.y;
+    f.nm = -st.x;
     auto one = [&](int64_t col) {
-      const float e = fast_exp(to_float(row[col]) + nm);
-      drow[col] = from_float<T>(col == t ? fmaf(a, e, c) : a * e);
+      drow[col] = from_float<T>(f.one(to_float(row[col]), col == t));
     };
-    const float2 nm2 = splat2(nm), a2 = splat2(a);
     auto vec = [&](const uint4& raw, int64_t v) {
-      float x[V];
-      unpack<T>(raw, x);
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2),
-                                    splat2(kLog2e));
-        x[e] = fast_exp2(y.x);
-        x[e + 1] = fast_exp2(y.y);
-      }
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float2 y = __fmul2_rn(make_float2(x[e], x[e + 1]), a2);
-        x[e] = y.x;
-        x[e + 1] = y.y;
-      }
-      st_stream(dbody + v * V, pack<T>(x));
+      st_stream(dbody + v * V, f.vec<T>(raw));
       // The thread that stored the target's vector stores the target's element over it.
       if ((uint64_t)(t - (head + v * V)) < (uint64_t)V) one(t);
     };
@@ -742,29 +855,89 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
     }
   }
   __syncthreads();
-  const float c = shared_row.z, a = -c * shared_row.y, nm = -shared_row.x;
-  auto one = [&](int64_t col, float x) {
-    const float e = fast_exp(x + nm);
-    drow[col] = from_float<T>(col == t ? fmaf(a, e, c) : a * e);
-  };
-  if (edge >= 0) one(edge, xe);
-  const float2 nm2 = splat2(nm), a2 = splat2(a);
+  const RowGrad f{-shared_row.z * shared_row.y, shared_row.z, -shared_row.x};
+  if (edge >= 0) drow[edge] = from_float<T>(f.one(xe, edge == t));
   // The target's vector in this slice, if it is here.
   const int64_t from = t - (head + part.v0 * V);
   const int tv = from >= 0 && from < (int64_t)n * V ? (int)(from / V) : -1;
 #pragma unroll 2
   for (int u = w0 + lane; u < w1; u += 32) {
-    float x[V];
-    unpack<T>(lds128(slice + (size_t)u * 16), x);
-#pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm2), splat2(kLog2e));
-      const float2 d = __fmul2_rn(make_float2(fast_exp2(y.x), fast_exp2(y.y)), a2);
-      x[e] = d.x;
-      x[e + 1] = d.y;
+    st_stream(dbody + (int64_t)u * V, f.vec<T>(lds128(slice + (size_t)u * 16)));
+    if (u == tv) drow[t] = from_float<T>(f.one(to_float(row[t]), true));
+  }
+}
+
+// The same for short rows: one warp per row, which stays in registers.
+template <typename T>
+__global__ void __launch_bounds__(kShortWarps * 32)
+policy_short_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t rows,
+                    int64_t vocab, PolicyTerms p, float grad, RowOut out,
+                    T* __restrict__ dlogits, RowGrid dg) {
+  constexpr int V = Vec16<T>::N;
+  constexpr int kHeld = kShortVecs / 32;  // vectors per lane
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kShortWarps + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const RowIndex index = tg.index(r);
+  const int64_t t = tg.at(index);
+  const RowKind kind = row_kind(t, tg.ignore, vocab);
+  const T* row = logits + lg.offset(index);
+  T* drow = dlogits + dg.offset(index);
+  const int head = head_elems(row, vocab);
+  const int nvec = (int)((vocab - head) / V);
+  const int64_t edge = edge_of(lane, head, head + (int64_t)nvec * V, vocab);
+  const T* body = row + head;
+  T* dbody = drow + head;
+  if (kind != kRowUsed) {
+    if (edge >= 0) drow[edge] = from_float<T>(0.0f);
+    for (int v = lane; v < nvec; v += 32) st_stream(dbody + v * V, make_uint4(0, 0, 0, 0));
+    if (lane == 0) {
+      out.store(r, kind, Stat{0.0f, 1.0f}, 0.0f);
+      p.term[r] = kind == kRowIgnored ? 0.0 : NAN;
+      p.coef[r] = 0.0f;
     }
-    st_stream(dbody + (int64_t)u * V, pack<T>(x));
-    if (u == tv) one(t, to_float(row[t]));
+    return;
+  }
+  uint4 raw[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (lane + 32 * u < nvec) raw[u] = ld_stream(body + (lane + 32 * u) * V);
+  PolicyRow terms;
+  terms.load(p, index);
+  const float xt = to_float(row[t]), xe = edge >= 0 ? to_float(row[edge]) : 0.0f;
+  Running acc;
+  if (edge >= 0) acc.add1(xe);
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    if (lane + 32 * u < nvec) {
+      float x[V];
+      unpack<T>(raw[u], x);
+      acc.template add<V>(x);
+    }
+  }
+  const Stat own = acc.stat();
+  Stat total;
+  total.m = warp_max(own.m);
+  total.s = warp_sum(sum_at(own, total.m));
+  double term;
+  float coef;
+  terms.term(p, log_softmax(total, xt), term, coef);
+  if (lane == 0) {
+    out.store(r, kind, total, xt);
+    p.term[r] = term;
+    p.coef[r] = coef;
+  }
+  const float c = coef * grad;
+  const RowGrad f{-c * (1.0f / total.s), c, -total.m};
+  if (edge >= 0) drow[edge] = from_float<T>(f.one(xe, edge == t));
+  const int tv = t >= head && t < head + (int64_t)nvec * V ? (int)((t - head) / V) : -1;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) {
+    const int v = lane + 32 * u;
+    if (v < nvec) {
+      st_stream(dbody + v * V, f.vec<T>(raw[u]));
+      if (v == tv) drow[t] = from_float<T>(f.one(xt, true));
+    }
   }
 }
 
@@ -803,8 +976,10 @@ struct Rows {  // the checked geometry of a call
   Targets tg;
 };
 
-// Splits of each row: one CTA a row when the rows alone fill the GPU, else so many that about
-// eight CTAs per SM share the work, each with at least one unrolled trip of 16-byte vectors.
+// Splits of each row for its statistics: one CTA a row when the rows alone fill the GPU, else so
+// many that about eight CTAs per SM share the work, each with at least one unrolled trip of
+// 16-byte vectors. (More splits, for a fuller last wave, gained 13 % at 1300 rows of 128256
+// bf16 logits and lost 8 to 20 % at other sizes.)
 int split_count(int64_t rows, int64_t vocab, int elem, int sms) {
   const int64_t trips = vocab * elem / 16 / (kThreads * kUnrollStats);
   const int64_t want = rows > 0 ? ((int64_t)sms * 8 + rows - 1) / rows : 1;
@@ -882,10 +1057,27 @@ int grid_of(int64_t items, int sms, int per_sm) {
 // One CTA per item, handed out as CTAs finish (items differ in length).
 int grid_of(int64_t items) { return (int)std::min<int64_t>(items, INT32_MAX); }
 
+// The longest rows, in 16-byte vectors, that one warp takes. Measured in bf16 against a CTA per row:
+// statistics of 65536 x 1000 / 16384 x 8000 / 8192 x 16000 logits 50 / 54 / 52 against 160 / 109 / 72
+// us (at 30000 logits even); gradient of 65536 x 1000 / 16384 x 8000 / 8192 x 16000 45 / 85 / 90
+// against 159 / 95 / 86 us; policy pass of 65536 x 1000 / 32768 x 4000 108 / 107 against 207 / 157.
+constexpr int kShortStatVecs = 2048;
+constexpr int kShortGradVecs = 1024;
+// Whether a warp takes a row: rows of at most `vecs` vectors that give every SM eight CTAs so.
+bool short_rows(const Rows& g, int elem, int vecs) {
+  return g.vocab * elem <= (int64_t)vecs * 16 && g.rows >= (int64_t)g.sms * 8 * kShortWarps;
+}
+unsigned short_grid(const Rows& g) { return (unsigned)((g.rows + kShortWarps - 1) / kShortWarps); }
+
 template <typename T>
 void launch_stats(const Rows& g, const void* logits, Stat* part, const RowOut& out,
                   cudaStream_t s) {
   const T* x = static_cast<const T*>(logits);
+  if (short_rows(g, sizeof(T), kShortStatVecs)) {
+    stats_short_kernel<T><<<short_grid(g), kShortWarps * 32, 0, s>>>(x, g.lg, g.tg, g.rows,
+                                                                     g.vocab, out);
+    return;
+  }
   stats_kernel<T><<<grid_of(g.rows * g.splits), kThreads, 0, s>>>(
       x, g.lg, g.tg, g.rows, g.vocab, g.splits, part, out);
   if (g.splits > 1)
@@ -971,9 +1163,34 @@ int cluster_size(int64_t rows, int64_t row_bytes, int sms) {
 }
 
 template <typename T>
+void launch_grad(const Rows& g, const void* logits, const float2* stats, const float* coef,
+                 const RowGrid& cg, const float* grad, void* dlogits, const RowGrid& dg,
+                 cudaStream_t s) {
+  const T* x = static_cast<const T*>(logits);
+  T* dx = static_cast<T*>(dlogits);
+  if (short_rows(g, sizeof(T), kShortGradVecs)) {
+    grad_short_kernel<T><<<short_grid(g), kShortWarps * 32, 0, s>>>(
+        x, g.lg, g.tg, g.rows, g.vocab, stats, coef, cg, grad, dx, dg);
+    return;
+  }
+  // kGradTrips unrolled trips per CTA, fewer (down to one) while that leaves SMs without eight CTAs.
+  const int64_t trips = g.vocab / Vec16<T>::N / (kGradThreads * kUnrollGrad);
+  const int64_t spread = std::min(trips, ((int64_t)g.sms * 8 + g.rows - 1) / g.rows);
+  const int splits = (int)std::max<int64_t>({1, trips / kGradTrips, spread});
+  grad_kernel<T><<<grid_of(g.rows * splits), kGradThreads, 0, s>>>(
+      x, g.lg, g.tg, g.rows, g.vocab, splits, stats, coef, cg, grad, dx, dg);
+}
+
+template <typename T>
 int launch_policy_grad(const Rows& g, const void* logits, int cluster, const PolicyTerms& p,
                        float grad, const RowOut& out, void* dlogits, const RowGrid& dg,
                        cudaStream_t s) {
+  if (short_rows(g, sizeof(T), kShortVecs)) {
+    policy_short_kernel<T><<<short_grid(g), kShortWarps * 32, 0, s>>>(
+        static_cast<const T*>(logits), g.lg, g.tg, g.rows, g.vocab, p, grad, out,
+        static_cast<T*>(dlogits), dg);
+    return PT_OK;
+  }
   // The largest slice: ceil(vectors / cluster) vectors (an unaligned row has fewer whole ones).
   const int64_t nvec = g.vocab / Vec16<T>::N;
   const size_t smem = (size_t)((nvec + cluster - 1) / cluster) * 16;
@@ -1086,27 +1303,11 @@ int pt_token_logps_bwd(const void* logits, int64_t vocab, int64_t outer, int64_t
   const RowGrid cg{coef_outer_stride, coef_inner_stride};
   const RowGrid dg{dlogits_outer_stride, dlogits_inner_stride};
   const float2* st2 = reinterpret_cast<const float2*>(stats);
-  // kGradTrips unrolled trips per CTA, fewer (down to one) while that leaves SMs without eight CTAs.
-  const int64_t trips = vocab * dtype_size(dtype) / 16 / (kGradThreads * kUnrollGrad);
-  const int64_t spread = std::min(trips, ((int64_t)g.sms * 8 + g.rows - 1) / g.rows);
-  const int splits = (int)std::max<int64_t>({1, trips / kGradTrips, spread});
-  const int grid = grid_of(g.rows * splits);
   cudaStream_t s = as_stream(stream);
   switch (dtype) {
-    case PT_FLOAT32:
-      grad_kernel<float><<<grid, kGradThreads, 0, s>>>(static_cast<const float*>(logits), g.lg, g.tg,
-                                                   g.rows, vocab, splits, st2, coef, cg, grad,
-                                                   static_cast<float*>(dlogits), dg);
-      break;
-    case PT_FLOAT16:
-      grad_kernel<__half><<<grid, kGradThreads, 0, s>>>(static_cast<const __half*>(logits), g.lg,
-                                                    g.tg, g.rows, vocab, splits, st2, coef, cg,
-                                                    grad, static_cast<__half*>(dlogits), dg);
-      break;
-    default:
-      grad_kernel<__nv_bfloat16><<<grid, kGradThreads, 0, s>>>(
-          static_cast<const __nv_bfloat16*>(logits), g.lg, g.tg, g.rows, vocab, splits, st2,
-          coef, cg, grad, static_cast<__nv_bfloat16*>(dlogits), dg);
+    case PT_FLOAT32: launch_grad<float>(g, logits, st2, coef, cg, grad, dlogits, dg, s); break;
+    case PT_FLOAT16: launch_grad<__half>(g, logits, st2, coef, cg, grad, dlogits, dg, s); break;
+    default: launch_grad<__nv_bfloat16>(g, logits, st2, coef, cg, grad, dlogits, dg, s);
   }
   return check_launch("pt_token_logps_bwd");
 }

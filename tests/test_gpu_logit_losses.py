@@ -635,6 +635,35 @@ def test_many_rows():
     _check_policy(x, t, old, adv, ref, 0.1, "sequence", scales=(None,))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab", [2, 9, 333, 1003, 2048, 4103, 8192])
+def test_many_short_rows(vocab, dtype):
+    """Enough rows that a warp takes a row each (4736 on B200), aligned and not, whole batches and
+    a slice of them, with rows that have no target and rows of every mask."""
+
+    shape = (5, 1201, vocab)
+    x, t = _data(shape, dtype, seed=54)
+    x[0, 0, 1:] = -math.inf
+    x[0, 2, :] = torch.finfo(dtype).min
+    t[0, :3] = 0
+    x[1, 1, :] = math.nan
+    t[1, 1] = IGNORE
+    clean = x.clone()
+    clean[1, 1] = 0.0
+    cut = (slice(None), slice(1, None))
+    for view in (slice(None), cut):
+        leaf = x[view].detach().requires_grad_()
+        lp = kernels.token_log_probs(leaf, t[view])
+        _check_logps(lp.detach(), clean[view], t[view])
+        dlp = gu.randn(t[view].shape, 55)
+        (dx,) = torch.autograd.grad(lp, leaf, dlp)
+        _check_grad(dx, clean[view], t[view], dlp)
+    old, ref, adv = _policy_inputs(clean, t, 56)
+    old[torch.isinf(old)] = -60.0
+    ref[torch.isinf(ref)] = -60.0
+    _check_policy(clean, t, old, adv, ref, 0.1, "sequence", scales=(None, 0.25))
+
+
 def test_offsets_beyond_32_bits():
     """Rows whose byte and element offsets pass 2^31 and 2^32."""
 
