@@ -48,6 +48,23 @@ struct Geom {
   float scale, sign;
 };
 
+// The angles of `count` tokens from token0 on: (c, s) per pair, by all threads of the CTA.
+__device__ __forceinline__ void fill_table(const Geom& g, float2* table, uint32_t token0,
+                                           uint32_t count) {
+  for (uint32_t i = threadIdx.x; i < count * g.half; i += kThreads) {
+    const uint32_t tok = g.div_half.div(i), p = i - tok * g.half;
+    const uint32_t b = g.div_s.div(token0 + tok), s = token0 + tok - b * g.div_s.d;
+    const double a = (double)g.positions[b * g.pb + s * g.ps] * g.inv_freq[p];
+    // a less whole turns, with 2 pi as a sum of two 64-bit numbers: exact to 64 bits for any a
+    // whose turns are whole numbers in 64 bits, where a fraction of a / (2 pi) loses |a| 2^-53.
+    const double turns = rint(a * 0.15915494309189535);
+    const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, a));
+    float sn, c;
+    sincospif((float)(rest * 0.3183098861837907), &sn, &c);
+    table[i] = make_float2(c * g.scale, g.sign * (sn * g.scale));
+  }
+}
+
 // N consecutive elements of T moved as one access of N * sizeof(T) bytes, as fp32.
 template <typename T, int N> struct Pack {
   static constexpr int kBytes = N * (int)sizeof(T);
@@ -201,18 +218,7 @@ rope_positions_kernel(const __grid_constant__ Geom g) {
       load(w[k], d[k]);
     }
   }
-  for (uint32_t i = threadIdx.x; i < count * g.half; i += kThreads) {
-    const uint32_t tok = kOne ? 0 : g.div_half.div(i), p = i - tok * g.half;
-    const uint32_t b = g.div_s.div(token0 + tok), s = token0 + tok - b * g.div_s.d;
-    const double a = (double)g.positions[b * g.pb + s * g.ps] * g.inv_freq[p];
-    // a less whole turns, with 2 pi as a sum of two 64-bit numbers: exact to 64 bits for any a
-    // whose turns are whole numbers in 64 bits, where a fraction of a / (2 pi) loses |a| 2^-53.
-    const double turns = rint(a * 0.15915494309189535);
-    const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, a));
-    float sn, c;
-    sincospif((float)(rest * 0.3183098861837907), &sn, &c);
-    table[i] = make_float2(c * g.scale, g.sign * (sn * g.scale));
-  }
+  fill_table(g, table, token0, count);
   __syncthreads();
   for (uint32_t u0 = threadIdx.x; u0 < total; u0 += kThreads * kUnits) {
     if (u0 != threadIdx.x) {
@@ -229,6 +235,131 @@ rope_positions_kernel(const __grid_constant__ Geom g) {
     for (int k = 0; k < kUnits; ++k)
       if (u0 + k * kThreads < total) finish(w[k], d[k]);
   }
+}
+
+// Rows path, for heads whose rows are not made of whole 16-byte vectors (head_dim 78 or 226 in
+// bf16, a boundary or a half at an odd place): where the heads of a token lie behind one
+// another, the token's row of heads x head_dim elements is one run of memory. It goes through
+// shared memory in 16-byte vectors, whatever its start, and the pairs are rotated there, one per
+// thread. The path above moves such heads in 8 to 2 bytes at a time and is bound by the address
+// arithmetic of each: for 16384 tokens of 20 + 5 heads of 78 (66 rotated) in bf16 it took 64
+// (interleaved) and 78 us (rotate-half), this one 46; for 10 + 5 heads of 226 107 and 115 us, this
+// one 86; for 14 + 2 heads of 96 (40 rotated, rotate-half) 35 us, this one 31. What bounds it now is
+// the instruction issue of the pairs. In fp32 the two take equally long, and the other is used.
+struct RowGeom {
+  uint32_t n[2];       // elements of a row: heads * head_dim
+  uint32_t vecs[2];    // vectors that a row touches, at most
+  uint32_t slot[2];    // where a token's rows start in shared memory (bytes)
+  uint32_t token_bytes;
+  uint32_t dim;
+  uint32_t step_pairs, step_heads;  // kThreads pairs on: so many whole heads and pairs
+  FastDiv div_vecs, div_pairs;  // by the vectors and by the pairs (of all heads) of one token
+};
+
+template <typename T, bool kRotateHalf>
+__global__ void __launch_bounds__(kThreads)
+rope_rows_positions_kernel(const __grid_constant__ Geom g, const __grid_constant__ RowGeom rg) {
+  constexpr int V = Vec16<T>::N;
+  constexpr int kLoads = 4;
+  struct Row {
+    const T* x;
+    T* out;
+    T* held;     // the row's first element in shared memory
+    int before;  // elements of its first vector that lie before it
+  };
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ Row rows[kMaxTokens * 2];
+  float2* table = reinterpret_cast<float2*>(shared + g.tokens_per_cta * rg.token_bytes);
+  const uint32_t token0 = blockIdx.x * g.tokens_per_cta;
+  const uint32_t count = min(g.tokens_per_cta, g.tokens - token0);
+  if (threadIdx.x < 2 * count) {
+    const uint32_t tok = threadIdx.x >> 1, i = threadIdx.x & 1;
+    const uint32_t b = g.div_s.div(token0 + tok), s = token0 + tok - b * g.div_s.d;
+    Row r;
+    r.x = static_cast<const T*>(g.x[i]) + (int64_t)b * g.xb[i] + (int64_t)s * g.xs[i];
+    r.out = static_cast<T*>(g.out[i]) + (int64_t)b * g.ob[i] + (int64_t)s * g.os[i];
+    r.before = (int)((reinterpret_cast<uintptr_t>(r.x) & 15u) / sizeof(T));
+    r.held = reinterpret_cast<T*>(shared + tok * rg.token_bytes + rg.slot[i]) + r.before;
+    rows[threadIdx.x] = r;
+  }
+  __syncthreads();
+
+  // Vector u of the CTA's rows: its row and first element; whole vectors only are moved as such.
+  auto whole = [&](uint32_t u, uint32_t& row, int& first) {
+    const uint32_t tok = rg.div_vecs.div(u);
+    const uint32_t in = u - tok * rg.div_vecs.d, i = in >= rg.vecs[0] ? 1 : 0;
+    row = 2 * tok + i;
+    first = (int)(in - (i ? rg.vecs[0] : 0)) * V - rows[row].before;
+    return first >= 0 && first + V <= (int)rg.n[i];
+  };
+  // The elements of a row before its first whole vector and behind its last, one per thread:
+  // `move` gets the row and the element.
+  auto edges = [&](auto move) {
+    for (uint32_t q = threadIdx.x; q < 2 * count * 2 * V; q += kThreads) {
+      const Row& r = rows[q / (2 * V)];
+      const int n = (int)rg.n[(q / (2 * V)) & 1], e = (int)(q % (2 * V));
+      const int head = min(n, (V - r.before) % V), tail = (n - head) % V;
+      if (e < head)
+        move(r, e);
+      else if (e >= V && e - V < tail)
+        move(r, n - tail + e - V);
+    }
+  };
+
+  const uint32_t vecs = count * rg.div_vecs.d;
+  for (uint32_t u0 = threadIdx.x; u0 < vecs; u0 += kThreads * kLoads) {
+    uint4 raw[kLoads];
+    T* at[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      uint32_t row;
+      int first;
+      at[k] = nullptr;
+      if (u0 + k * kThreads < vecs && whole(u0 + k * kThreads, row, first)) {
+        at[k] = rows[row].held + first;
+        raw[k] = ld_stream(rows[row].x + first);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k)
+      if (at[k] != nullptr) *reinterpret_cast<uint4*>(at[k]) = raw[k];
+  }
+  edges([](const Row& r, int e) { r.held[e] = r.x[e]; });
+  fill_table(g, table, token0, count);
+  __syncthreads();
+  // Pair u = (token, head, pair of the head); the next one of a thread is kThreads further on.
+  const uint32_t pairs = count * rg.div_pairs.d;
+  uint32_t tok = rg.div_pairs.div(threadIdx.x);
+  uint32_t h = g.div_half.div(threadIdx.x - tok * rg.div_pairs.d);
+  uint32_t j = threadIdx.x - tok * rg.div_pairs.d - h * g.half;
+#pragma unroll 2
+  for (uint32_t u = threadIdx.x; u < pairs; u += kThreads) {
+    const uint32_t i = h >= g.heads0 ? 1 : 0;
+    T* a = rows[2 * tok + i].held + (h - (i ? g.heads0 : 0)) * rg.dim + (kRotateHalf ? j : 2 * j);
+    T* b = a + (kRotateHalf ? g.half : 1);
+    const float2 cs = table[tok * g.half + j];
+    const float x = to_float(*a), y = to_float(*b);
+    *a = from_float<T>(fmaf(x, cs.x, -(y * cs.y)));
+    *b = from_float<T>(fmaf(x, cs.y, y * cs.x));
+    j += rg.step_pairs;
+    h += rg.step_heads;
+    if (j >= g.half) {
+      j -= g.half;
+      ++h;
+    }
+    while (h >= g.heads) {
+      h -= g.heads;
+      ++tok;
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (uint32_t u = threadIdx.x; u < vecs; u += kThreads) {
+    uint32_t row;
+    int first;
+    if (whole(u, row, first)) st_stream(rows[row].out + first, lds128(rows[row].held + first));
+  }
+  edges([](const Row& r, int e) { r.out[e] = r.held[e]; });
 }
 
 struct Side {
@@ -289,12 +420,66 @@ int launch(Geom& g, int64_t D, int64_t R, bool rh, cudaStream_t s) {
   return check_launch("pt_rope_positions");
 }
 
-// The widest access that fits: 16, 8 or 4 bytes, else single elements.
+// Whether the rows path can take the call: the heads of a token behind one another in inputs and
+// outputs, whose rows start at the same place of a 16-byte vector, and one token's rows in kRowBytes.
+constexpr int64_t kRowBytes = 40 * 1024;
+template <typename T> bool make_rows(RowGeom& rg, const Side* sides, int64_t D, int64_t R) {
+  constexpr int elem = (int)sizeof(T);
+  int64_t at = 0;
+  for (int i = 0; i < 2; ++i) {
+    const Side& t = sides[i];
+    const int64_t H = t.sizes[1];
+    if (H > 0) {
+      if (H > 1 && (t.xst[1] != D || t.ost[1] != D)) return false;
+      if ((reinterpret_cast<uintptr_t>(t.x) - reinterpret_cast<uintptr_t>(t.out)) % 16) return false;
+      for (int a : {0, 2})
+        if (t.sizes[a] > 1 && (t.xst[a] - t.ost[a]) * elem % 16) return false;
+    }
+    if (H > kRowBytes || H * D * elem > kRowBytes) return false;
+    rg.n[i] = (uint32_t)(H * D);
+    rg.vecs[i] = H > 0 ? (uint32_t)((H * D * elem + 15) / 16 + 1) : 0;
+    rg.slot[i] = (uint32_t)at;
+    at += (int64_t)rg.vecs[i] * 16;
+  }
+  if (at + R / 2 * 8 > kRowBytes) return false;
+  rg.token_bytes = (uint32_t)at;
+  rg.dim = (uint32_t)D;
+  rg.div_vecs = FastDiv(rg.vecs[0] + rg.vecs[1]);
+  return true;
+}
+
+template <typename T>
+int launch_rows(Geom& g, RowGeom& rg, int64_t R, bool rh, cudaStream_t s) {
+  g.half = (uint32_t)(R / 2);
+  g.div_half = FastDiv(g.half);
+  rg.div_pairs = FastDiv(g.heads * g.half);
+  rg.step_pairs = kThreads % g.half;
+  rg.step_heads = kThreads / g.half;
+  // Tokens for four vectors a thread, as far as 16 KB (or one token) hold them.
+  const int64_t bytes = rg.token_bytes + (int64_t)g.half * 8;
+  const int64_t want = kThreads * 4 / rg.div_vecs.d;
+  const int64_t room = 16 * 1024 / bytes;
+  g.tokens_per_cta = (uint32_t)std::max<int64_t>(
+      1, std::min<int64_t>({want, room, kMaxTokens, (int64_t)g.tokens}));
+  const unsigned grid = (g.tokens + g.tokens_per_cta - 1) / g.tokens_per_cta;
+  const size_t smem = (size_t)(g.tokens_per_cta * bytes);
+  if (rh)
+    rope_rows_positions_kernel<T, true><<<grid, kThreads, smem, s>>>(g, rg);
+  else
+    rope_rows_positions_kernel<T, false><<<grid, kThreads, smem, s>>>(g, rg);
+  return check_launch("pt_rope_positions");
+}
+
+// The widest access that fits: 16 bytes, rows through shared memory (16-bit types), 8 or 4 bytes,
+// else single elements.
 template <typename T>
 int dispatch(Geom& g, const Side* sides, int64_t D, int64_t R, bool rh, cudaStream_t s) {
   constexpr int elem = (int)sizeof(T);
   constexpr int kWide = 16 / elem;
   if (fits(sides, D, R, kWide, elem, rh)) return launch<T, kWide>(g, D, R, rh, s);
+  [[maybe_unused]] RowGeom rg;
+  if constexpr (elem == 2)
+    if (make_rows<T>(rg, sides, D, R)) return launch_rows<T>(g, rg, R, rh, s);
   if (fits(sides, D, R, kWide / 2, elem, rh)) return launch<T, kWide / 2>(g, D, R, rh, s);
   if constexpr (elem == 2) {
     if (fits(sides, D, R, 2, elem, rh)) return launch<T, 2>(g, D, R, rh, s);

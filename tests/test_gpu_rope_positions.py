@@ -89,6 +89,28 @@ def test_layouts_sizes_and_types(b, s, hq, hk, d, r, layout, dtype):
     _run(q, k, _positions((b, s)), inv_freq, layout, 1.25)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("s,hq,hk,d,r", [
+    (1, 1, 1, 2, 2), (5, 1, 1, 6, 4), (700, 3, 1, 10, 10), (33, 20, 5, 78, 66), (300, 1, 2, 30, 2),
+    (9, 7, 3, 226, 226), (3, 129, 1, 22, 14), (1, 2, 1, 4094, 4094), (2, 60, 0, 78, 40),
+    (3, 250, 1, 82, 82),
+], ids=str)
+def test_rows_of_odd_heads(s, hq, hk, d, r, layout, dtype):
+    """Heads that are no whole 16-byte vectors, in rows that start anywhere: the attention layer's
+    view, a slice of a fused projection (whose rows the gradient's do not match) and one token."""
+
+    fused = gu.randn((2, s, (hq + hk) * d), 1, dtype)
+    q = fused[..., : hq * d].unflatten(-1, (hq, d)).transpose(1, 2)
+    k = fused[..., hq * d:].unflatten(-1, (hk, d)).transpose(1, 2)
+    inv_freq, _ = rotary_frequencies(r, device=gu.DEV)
+    pos = _positions((2, s))
+    a = _run(q, k, pos, inv_freq, layout, 0.75)
+    b = _run(q.transpose(1, 2).contiguous().transpose(1, 2),
+             k.transpose(1, 2).contiguous().transpose(1, 2), pos, inv_freq, layout, 0.75)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def _shifted(shape, seed, dtype, shift):
     """A dense tensor that starts `shift` elements into its storage."""
 
