@@ -664,6 +664,17 @@ def test_many_short_rows(vocab, dtype):
     _check_policy(clean, t, old, adv, ref, 0.1, "sequence", scales=(None, 0.25))
 
 
+@pytest.mark.parametrize("aggregate", ["token", "sequence"])
+@pytest.mark.parametrize("shape", [(3, 30000, 12), (9000, 9, 12)], ids=str)
+def test_policy_weights_of_many_tokens(shape, aggregate):
+    """More tokens than one CTA counts, in few sequences and in many, some without a target."""
+
+    x, t = _data(shape, torch.float32, seed=57)
+    t[::3] = IGNORE
+    old, ref, adv = _policy_inputs(x, t, 58)
+    _check_policy(x, t, old, adv, ref, 0.1, aggregate, scales=(None,))
+
+
 def test_offsets_beyond_32_bits():
     """Rows whose byte and element offsets pass 2^31 and 2^32."""
 
