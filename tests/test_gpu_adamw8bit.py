@@ -211,9 +211,8 @@ def test_more_tensors_than_one_launch_and_per_tensor_scalars():
         assert torch.equal(p, got) and all(torch.equal(a, b) for a, b in zip(s, state))
 
 
-def test_tracks_32_bit_adamw():
-    """200 steps on a quadratic: the 8-bit run stays near torch's. An example tested for its
-    first steps only: the first update of AdamW is lr * sign(g) whatever the states hold."""
+def test_first_step_is_32_bit_adamws():
+    """The first update of AdamW is lr * sign(g) whatever precision the states are kept in."""
 
     p8 = torch.nn.Parameter(gu.randn((64, 40), 3))
     p32 = torch.nn.Parameter(p8.detach().clone())
