@@ -635,14 +635,17 @@ struct PolicyRow {
   }
   // max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
   // derivative to lp: -A r where the unclipped term is the larger one, and kl (1 - e^g). The
-  // differences are taken in 64 bits, the exponentials of these small numbers in 32.
+  // differences are taken in 64 bits, the exponentials of these small numbers in 32. NaN of any
+  // input is kept in both (fmaxf and fminf return their other operand, so comparisons that it
+  // fails choose here).
   __device__ __forceinline__ void term(const PolicyTerms& p, double lp, double& term,
                                        float& coef) const {
     const float r = expf((float)(lp - (double)old));
-    const bool inside = adv > 0.0f ? r <= p.high : r >= p.low;
-    const float gain = -adv * r;
-    double value = fmaxf(gain, -adv * fminf(fmaxf(r, p.low), p.high));
-    double slope = inside ? gain : 0.0f;
+    const float clipped = r < p.low ? p.low : r > p.high ? p.high : r;
+    const float gain = -adv * r, bounded = -adv * clipped;
+    const bool beyond = adv > 0.0f ? r > p.high : r < p.low;
+    double value = gain <= bounded ? bounded : gain;
+    double slope = value != value ? value : beyond ? 0.0 : gain;
     if (p.ref != nullptr) {
       const double g = (double)ref - lp;
       const float eg = expm1f((float)g);

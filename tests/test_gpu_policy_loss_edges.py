@@ -1,0 +1,119 @@
+"""policy_loss on inputs that are not numbers, and on what else its callers may hand it: NaN and
+infinities in every input, targets outside the vocabulary, ratios beyond the range of 32 bits,
+gradients that are not finite, and a backward pass that is captured by itself.
+
+Rows are compared bit for bit with those of a call on clean inputs: a row's gradient depends on
+that row and on the number of positions with a target alone.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import gpu_utils as gu
+from picotron_b200 import _capi, kernels
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+AT = (0, 2)  # the row that is broken; it has a target
+# A path of the implementation: shape, dtype, whether the logits need a gradient, and what
+# expected_grad is given. float16 without a hint forms its gradient in backward.
+PATHS = {
+    "one pass": ((2, 5, 1003), torch.bfloat16, True, None),
+    "one pass, a cluster per row": ((1, 3, 100_003), torch.float32, True, None),
+    "two passes": ((2, 5, 1003), torch.float16, True, None),
+    "no gradient": ((2, 5, 1003), torch.float32, False, None),
+    "many short rows": ((3, 2000, 37), torch.bfloat16, True, None),
+    "many short rows, two passes": ((3, 2000, 37), torch.float16, True, None),
+}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    gu.require_gpu()
+    _capi.take_device_error()
+
+
+def _inputs(shape, dtype):
+    g = torch.Generator().manual_seed(5)
+    x = (torch.randn(shape, generator=g) * 2.0).to(dtype).to(gu.DEV)
+    t = torch.randint(0, shape[-1], shape[:2], generator=g)
+    t.view(-1)[1::4] = IGNORE
+    t = t.to(gu.DEV)
+    old = kernels.token_log_probs(x, t) + 0.01  # ratios next to 1, inside the clipping range
+    return x, t, old, old - 0.02, gu.randn(shape[:2], 6) + 3.0
+
+
+def _call(x, t, old, ref, adv, kl, path):
+    _, _, grad, expected = PATHS[path]
+    leaf = x.detach().requires_grad_(grad)
+    loss, lp = kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref if kl else None,
+                                   kl_coef=kl, expected_grad=expected)
+    dx = torch.autograd.grad(loss, leaf)[0] if grad else None
+    return loss.detach(), lp, dx
+
+
+def _set(tensor, value):
+    out = tensor.clone()
+    out[AT] = value
+    return out
+
+
+BREAK = {
+    "NaN among the logits": lambda x, t, old, ref, adv: (_at(x, 7, math.nan), t, old, ref, adv),
+    "infinite logit": lambda x, t, old, ref, adv: (_at(x, 7, math.inf), t, old, ref, adv),
+    "no finite logit": lambda x, t, old, ref, adv: (_set(x, -math.inf), t, old, ref, adv),
+    "NaN old": lambda x, t, old, ref, adv: (x, t, _set(old, math.nan), ref, adv),
+    "NaN advantage": lambda x, t, old, ref, adv: (x, t, old, ref, _set(adv, math.nan)),
+    "NaN reference": lambda x, t, old, ref, adv: (x, t, old, _set(ref, math.nan), adv),
+    "both -inf": lambda x, t, old, ref, adv: (
+        _at(x, int(t[AT]), -math.inf), t, _set(old, -math.inf), ref, adv),
+}
+
+
+def _at(x, column, value):
+    out = x.clone()
+    out[(*AT, column)] = value
+    return out
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+@pytest.mark.parametrize("broken", BREAK)
+@pytest.mark.parametrize("path", PATHS)
+def test_what_is_not_a_number_stays_so(path, broken, kl):
+    clean = _inputs(*PATHS[path][:2])
+    for sign in (1.0, -1.0):
+        args = [*clean[:4], clean[4] * sign]
+        want_loss, _, want = _call(*args, kl, path)
+        loss, _, dx = _call(*BREAK[broken](*args), kl, path)
+        if broken == "NaN reference" and not kl:  # not read
+            assert torch.equal(loss, want_loss) and (dx is None or torch.equal(dx, want))
+            continue
+        assert torch.isfinite(want_loss) and torch.isnan(loss)
+        if dx is not None:
+            assert torch.isnan(dx[AT]).all()
+            rest = torch.ones(dx.shape[:2], dtype=torch.bool, device=gu.DEV)
+            rest[AT] = False
+            assert torch.equal(dx[rest], want[rest])
+    assert _capi.take_device_error() == 0
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+@pytest.mark.parametrize("target", [-1, "vocab"])
+@pytest.mark.parametrize("path", PATHS)
+def test_a_target_outside_the_vocabulary(path, target, kl):
+    x, t, old, ref, adv = _inputs(*PATHS[path][:2])
+    _, _, want = _call(x, t, old, ref, adv, kl, path)
+    bad = _set(t, x.size(-1) if target == "vocab" else target)
+    loss, lp, dx = _call(x, bad, old, ref, adv, kl, path)
+    assert torch.isnan(loss) and torch.isnan(lp[AT])
+    if dx is not None:
+        assert (dx[AT] == 0).all()
+        want = want.clone()
+        want[AT] = 0
+        assert torch.equal(dx, want)
+    assert _capi.take_device_error() == 2 and _capi.take_device_error() == 0
