@@ -617,11 +617,14 @@ struct PolicyTerms {
   const float* ref;  // null without a KL term
   RowGrid rg;
   const double* weight;  // [outer]
-  float low, high;       // 1 - clip_low, 1 + clip_high
-  float kl;
+  double low, high;      // 1 - clip_low, 1 + clip_high
+  double kl;
   double* term;     // [rows] weighted loss terms
   float* coef;      // [rows] d loss / d logp
 };
+
+constexpr double kOrdinary = 2.0;
+__device__ __noinline__ double far_exp(double x) { return exp(x); }
 
 // What a row's loss term takes besides its log-probability.
 struct PolicyRow {
@@ -633,24 +636,37 @@ struct PolicyRow {
     ref = p.ref != nullptr ? p.ref[p.rg.offset(i)] : 0.0f;
     weight = p.weight[i.outer];
   }
-  // max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
-  // derivative to lp: -A r where the unclipped term is the larger one, and kl (1 - e^g). The
-  // differences are taken in 64 bits, the exponentials of these small numbers in 32. NaN of any
-  // input is kept in both (fmaxf and fminf return their other operand, so comparisons that it
-  // fails choose here).
+  // max(-A r, -A clip(r)) and its derivative to lp: -A r where the unclipped term is the larger
+  // one. NaN of any input is kept in both (fmax and fmin return their other operand, so comparisons
+  // that it fails choose here).
+  template <typename F>
+  static __device__ __forceinline__ void clip(F r, F a, F low, F high, double& value,
+                                              double& slope) {
+    const F clipped = r < low ? low : r > high ? high : r;
+    const F gain = -a * r, bounded = -a * clipped;
+    const bool beyond = a > F(0) ? r > high : r < low;
+    const F larger = gain <= bounded ? bounded : gain;
+    value = larger;
+    slope = larger != larger ? larger : beyond ? F(0) : gain;
+  }
+  // The clipped term of r = e^(lp - old) and kl (e^g - g - 1) of g = ref - lp, whose derivative is
+  // kl (1 - e^g). The differences are taken in 64 bits. Exponentials of up to kOrdinary are taken
+  // in 32 bits: expf is within 2^-22 and expm1f within 2^-22 |e^g - 1| there, which is what an
+  // error of 2^-22 in the log-probability makes of r and of the KL term. Larger arguments are taken
+  // in 64 bits, where e^89 and above are finite, so that a zero advantage weighs nothing.
   __device__ __forceinline__ void term(const PolicyTerms& p, double lp, double& term,
                                        float& coef) const {
-    const float r = expf((float)(lp - (double)old));
-    const float clipped = r < p.low ? p.low : r > p.high ? p.high : r;
-    const float gain = -adv * r, bounded = -adv * clipped;
-    const bool beyond = adv > 0.0f ? r > p.high : r < p.low;
-    double value = gain <= bounded ? bounded : gain;
-    double slope = value != value ? value : beyond ? 0.0 : gain;
+    const double d = lp - (double)old;
+    double value, slope;
+    if (fabs(d) <= kOrdinary)
+      clip(expf((float)d), adv, (float)p.low, (float)p.high, value, slope);
+    else
+      clip(far_exp(d), (double)adv, p.low, p.high, value, slope);
     if (p.ref != nullptr) {
       const double g = (double)ref - lp;
-      const float eg = expm1f((float)g);
-      value += (double)p.kl * ((double)eg - g);
-      slope -= (double)p.kl * (double)eg;
+      const double eg = fabs(g) <= kOrdinary ? (double)expm1f((float)g) : far_exp(g) - 1.0;
+      value += p.kl * (eg - g);
+      slope -= p.kl * eg;
     }
     term = value * weight;
     coef = (float)(slope * weight);
@@ -1149,9 +1165,9 @@ int check_policy(Rows& g, Workspace& w, PolicyTerms& p, const PolicyInputs& in,
   p.ref = in.ref;
   p.rg = RowGrid{in.ro, in.ri};
   p.weight = w.seq;
-  p.low = (float)(1.0 - in.low);
-  p.high = (float)(1.0 + in.high);
-  p.kl = (float)in.kl;
+  p.low = 1.0 - in.low;
+  p.high = 1.0 + in.high;
+  p.kl = in.kl;
   p.term = w.term;
   p.coef = coef;
   return PT_OK;

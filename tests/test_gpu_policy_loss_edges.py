@@ -117,3 +117,37 @@ def test_a_target_outside_the_vocabulary(path, target, kl):
         want[AT] = 0
         assert torch.equal(dx, want)
     assert _capi.take_device_error() == 2 and _capi.take_device_error() == 0
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_ratios_beyond_the_range_of_32_bits(path):
+    """exp(logp - old) above 3.4e38: a zero advantage still costs nothing, a positive one is
+    clipped, and a negative one weighs a finite product."""
+
+    x, t, old, ref, adv = _inputs(*PATHS[path][:2])
+    n = int((t != IGNORE).sum())
+    lp = kernels.token_log_probs(x, t)
+    old = lp.clone()  # every other ratio is 1 up to the rounding of its log-probability
+    old[AT] = -100.0 + lp[AT].double().item()
+    exact = math.exp(lp[AT].double().item() - float(old[AT]))
+    for a, loss64, coef64 in ((0.0, 0.0, 0.0), (2.0, -2.4, 0.0),
+                              (-1e-30, 1e-30 * exact, 1e-30 * exact)):
+        advantages = _set(torch.zeros_like(adv), a)
+        loss, _, dx = _call(x, t, old, ref, advantages, 0.0, path)
+        # The log-probability is known to 2^-24 of itself, the loss is rounded once (2^-24), and a
+        # softmax value is off by 2 eps: its exponential by 2^-22 + 146 * 2^-24, its sum by
+        # V / 256 + 56 roundings more.
+        lp_error = 2.0 ** -22 + 2.0 ** -24 * abs(lp[AT].item())
+        eps = 2.0 ** -22 + 2.0 ** -24 * (x.size(-1) / 256 + 202)
+        assert abs(loss.item() - loss64 / n) <= 2 * lp_error * abs(loss64) / n
+        if dx is None:
+            continue
+        hot = torch.zeros(x.size(-1), dtype=torch.float64, device=gu.DEV)
+        hot[t[AT]] = 1.0
+        want = coef64 / n * (hot - torch.softmax(x[AT].double(), -1))
+        info = torch.finfo(x.dtype)
+        tol = ((2 * lp_error + 2 * eps) * abs(coef64) / n + want.abs() * info.eps
+               + info.smallest_normal)
+        fits = want.abs() < info.max  # float16 has no such gradients
+        assert ((dx[AT].double() - want).abs()[fits] <= tol[fits]).all()
+        assert (dx[t == IGNORE] == 0).all()
