@@ -189,6 +189,25 @@ def _rotate_part(states: Tensor, cosine: Tensor, sine: Tensor) -> Tensor:
     return torch.cat((out.flatten(start_dim=-2).to(states.dtype), states[..., rotated:]), dim=-1)
 
 
+def _kept(cache: dict[tuple, tuple], key: tuple, build) -> tuple:
+    """``cache[key]``, built on first use. What is kept serves calls in every mode: inference
+    tensors, which autograd cannot save, are built again as normal ones, and fake tensors or
+    tensors that a CUDA graph under capture has yet to fill are returned but not kept."""
+
+    held = cache.get(key)
+    if torch.compiler.is_compiling():  # what follows cannot be traced
+        if held is None:
+            held = cache[key] = build()
+        return held
+    if held is None or (held[0].is_inference() and not torch.is_inference_mode_enabled()):
+        with torch.inference_mode(False):
+            held = build()
+        if type(held[0]) is Tensor and not (held[0].is_cuda
+                                            and torch.cuda.is_current_stream_capturing()):
+            cache[key] = held
+    return held
+
+
 class RotaryEmbedding(nn.Module):
     """Apply (interleaved-pair) RoPE to attention query and key tensors.
 
@@ -220,13 +239,8 @@ class RotaryEmbedding(nn.Module):
 
     def _cos_sin(self, sequence_length: int, device: torch.device, dtype: torch.dtype):
         key = (sequence_length, str(device), dtype)
-        tables = self._tables.get(key)
-        if tables is None:
-            tables = rotary_cos_sin(
-                sequence_length, self.head_dim, self.theta, device=device, dtype=dtype
-            )
-            self._tables[key] = tables
-        return tables
+        return _kept(self._tables, key, lambda: rotary_cos_sin(
+            sequence_length, self.head_dim, self.theta, device=device, dtype=dtype))
 
     def _inverse_frequencies(self, device: torch.device) -> tuple[Tensor, float]:
         """rotary_frequencies of the module's settings, built once per setting and device."""
@@ -236,10 +250,8 @@ class RotaryEmbedding(nn.Module):
             raise ValueError("rotary_dim must be at most the attention head dimension.")
         scaling = self.scaling or {}
         key = (rotary_dim, self.theta, tuple(sorted(scaling.items())), str(device))
-        if key not in self._frequencies:
-            self._frequencies[key] = rotary_frequencies(rotary_dim, self.theta, device=device,
-                                                        **scaling)
-        return self._frequencies[key]
+        return _kept(self._frequencies, key, lambda: rotary_frequencies(
+            rotary_dim, self.theta, device=device, **scaling))
 
     def _by_positions(self, query: Tensor, key: Tensor,
                       positions: Tensor | None) -> tuple[Tensor, Tensor]:
