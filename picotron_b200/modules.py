@@ -237,6 +237,11 @@ class RotaryEmbedding(nn.Module):
         self._tables: dict[tuple, tuple[Tensor, Tensor]] = {}
         self._frequencies: dict[tuple, tuple[Tensor, float]] = {}
 
+    def __setstate__(self, state: dict) -> None:
+        """Modules that were pickled whole before there were positions lack what those need."""
+
+        super().__setstate__({"rotary_dim": None, "scaling": None, "_frequencies": {}, **state})
+
     def _cos_sin(self, sequence_length: int, device: torch.device, dtype: torch.dtype):
         key = (sequence_length, str(device), dtype)
         return _kept(self._tables, key, lambda: rotary_cos_sin(

@@ -3,6 +3,9 @@ call in any other mode."""
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -52,3 +55,20 @@ def test_fake_tensors_are_not_kept(setting):
     for a, b in zip(rope(q, k, positions), other(q, k, positions)):
         assert type(a) is torch.Tensor and torch.equal(a, b)
 
+
+def test_modules_from_before_positions_still_run():
+    """A module that was pickled whole by a version without the attributes for explicit
+    positions, and one that has them."""
+
+    rope = pb.RotaryEmbedding(16)
+    old = pb.RotaryEmbedding.__new__(pb.RotaryEmbedding)
+    old.__setstate__({name: value for name, value in rope.__dict__.items()
+                      if name not in ("rotary_dim", "scaling", "_frequencies")})
+    q, k = _states()
+    for positions in (None, torch.arange(6)):
+        for a, b in zip(old(q, k, positions), rope(q, k, positions)):
+            assert torch.equal(a, b)
+    rope.rotary_dim = 8
+    for twin in (copy.deepcopy(rope), pickle.loads(pickle.dumps(rope))):
+        assert twin.rotary_dim == 8
+        assert torch.equal(twin(q, k)[0], rope(q, k)[0])
