@@ -806,29 +806,38 @@ def _ll_workspace(logits: Tensor, outer: int, inner: int) -> Tensor:
     return torch.empty(size, dtype=torch.uint8, device=logits.device)
 
 
-def _ll_dense_gradient(logits: Tensor) -> bool:
-    """Whether a contiguous gradient's rows sit at the same offsets modulo 16 bytes."""
+def _ll_gradient_strides(logits: Tensor) -> tuple[int, ...] | None:
+    """Strides of a gradient whose rows sit at the logits' offsets modulo 16 bytes, or None where
+    those of a contiguous one do. The rows of a strided view of odd-sized rows keep the view's
+    strides while its span is less than twice the gradient's size; else they are padded to the
+    next such offset (the last position of 8 x 4096 x 50257 bf16 logits spans 2.9 GB)."""
 
-    size = logits.element_size()
-    return logits.is_contiguous() or all(
-        n * size % 16 == 0
-        for n in (logits.size(-1), *(logits.stride(d) for d in range(logits.dim() - 1)
-                                     if logits.size(d) > 1)))
+    if logits.is_contiguous():
+        return None
+    shape, strides, per = logits.shape, logits.stride(), 16 // logits.element_size()
+    leading = [d for d in range(logits.dim() - 1) if shape[d] > 1]
+    if all(n % per == 0 for n in (shape[-1], *(strides[d] for d in leading))):
+        return None
+    if 1 + sum((shape[d] - 1) * strides[d] for d in (*leading, -1)) < 2 * logits.numel():
+        return strides
+    padded, reach = [1], shape[-1]
+    for d in reversed(range(logits.dim() - 1)):
+        padded.append(reach + (strides[d] - reach) % per)
+        reach = padded[-1] * shape[d]
+    return tuple(reversed(padded))
 
 
 def _ll_gradient(logits: Tensor) -> Tensor:
     """An empty gradient whose rows have the addresses of the logits' rows modulo 16 bytes, so that
-    both are read and written in the same whole vectors: contiguous, or with the strides of a
-    strided view of odd-sized rows."""
+    both are read and written in the same whole vectors."""
 
     shift = logits.data_ptr() % 16 // logits.element_size()
-    dense = _ll_dense_gradient(logits)
-    if dense and shift == 0:
+    strides = _ll_gradient_strides(logits)
+    if strides is None and shift == 0:
         return torch.empty_like(logits, memory_format=torch.contiguous_format)
-    if dense:
+    if strides is None:
         buffer = torch.empty(logits.numel() + shift, dtype=logits.dtype, device=logits.device)
         return buffer[shift:].view(logits.shape)
-    strides = logits.stride()
     span = 1 + sum((n - 1) * st for n, st in zip(logits.shape, strides))
     buffer = torch.empty(span + shift, dtype=logits.dtype, device=logits.device)
     return buffer.as_strided(logits.shape, strides, shift)
@@ -896,9 +905,10 @@ def _ll_backward_of(ctx_tensors, grad, ignore_index) -> Tensor:
 
 def _logit_loss_backward_fake(logits, targets, stats, coef, grad, ignore_index):
     x = _ll_logits(logits)
-    if _ll_dense_gradient(x):
+    strides = _ll_gradient_strides(x)
+    if strides is None:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    return torch.empty_strided(x.shape, x.stride(), dtype=x.dtype, device=x.device)
+    return torch.empty_strided(x.shape, strides, dtype=x.dtype, device=x.device)
 
 
 logit_loss_backward = _Op(
