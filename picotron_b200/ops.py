@@ -1091,6 +1091,7 @@ class _PolicyLoss(torch.autograd.Function):
         else:
             loss, *rest, ctx.dlogits = policy_loss_grad.below(logits, targets, *args,
                                                        ctx.expected)
+            ctx.captured = torch.cuda.is_current_stream_capturing()
         logps, stats, coef = rest
         ctx.save_for_backward(logits, targets, stats, coef)
         ctx.ignore_index = args[-1]
@@ -1105,6 +1106,11 @@ class _PolicyLoss(torch.autograd.Function):
             return (None,) * 11
         logits, targets, stats, coef = ctx.saved_tensors
         dlogits, ctx.dlogits = ctx.dlogits, None
+        # A graph that captures the backward alone may be replayed: rescaling in place would be
+        # repeated on its own result.
+        if (dlogits is not None and not ctx.captured
+                and torch.cuda.is_current_stream_capturing()):
+            dlogits = None
         if dlogits is None:  # two passes, or a second backward through a retained graph
             dlogits = _ll_backward_of((logits, targets, stats, coef), grad, ctx.ignore_index)
         elif dlogits.numel():

@@ -151,3 +151,61 @@ def test_ratios_beyond_the_range_of_32_bits(path):
         fits = want.abs() < info.max  # float16 has no such gradients
         assert ((dx[AT].double() - want).abs()[fits] <= tol[fits]).all()
         assert (dx[t == IGNORE] == 0).all()
+
+
+def test_a_backward_that_is_captured_by_itself_can_be_replayed():
+    """The forward ran outside of the graph: its gradient, formed for another factor than it gets,
+    must not be rescaled once more by every replay."""
+
+    x, t, old, ref, adv = _inputs(*PATHS["one pass"][:2])
+    leaf = x.detach().requires_grad_()
+    up = torch.tensor(2.0, device=gu.DEV)
+
+    def loss():
+        return kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref, kl_coef=0.1)[0]
+
+    (want,) = torch.autograd.grad(loss(), leaf, up)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(loss(), leaf, up)
+        kept = loss()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (dx,) = torch.autograd.grad(kept, leaf, up)
+    results = []
+    for _ in range(3):
+        graph.replay()
+        results.append(dx.clone())
+    up.fill_(4.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    for got in results:
+        assert torch.equal(got, want)  # twice a bf16 value: no rounding on either way
+    assert torch.equal(dx, 2.0 * want)
+
+
+def test_a_forward_and_backward_that_are_captured_together_can_be_replayed():
+    x, t, old, ref, adv = _inputs(*PATHS["one pass"][:2])
+    leaf = x.detach().requires_grad_()
+    up = torch.tensor(2.0, device=gu.DEV)
+
+    def step():
+        loss, _ = kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref, kl_coef=0.1)
+        return torch.autograd.grad(loss, leaf, up)[0]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        dx = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
