@@ -483,7 +483,7 @@ PT_API int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer,
 
 /* Multiplies a gradient that was formed for the factor `expected` (finite, not 0) by *grad /
  * expected, in place; *grad is one fp32 value in device memory, and where it equals expected
- * nothing is read or written. */
+ * nothing is read or written. Zeros stay zeros, also where *grad is not finite. */
 PT_API int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t inner,
                                   int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
                                   const float* grad, double expected, int dtype, void* stream);

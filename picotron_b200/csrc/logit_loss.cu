@@ -964,7 +964,9 @@ policy_short_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_
   }
 }
 
-// dx *= grad / expected, unless they are equal.
+// dx *= grad / expected, unless they are equal. Zeros stay zeros, also where the factor is not
+// finite: rows without a target have no gradient whatever the loss's is.
+__device__ __forceinline__ float rescaled(float x, float f) { return x != 0.0f ? x * f : x; }
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 rescale_kernel(T* __restrict__ dlogits, RowGrid dg, RowDiv index, int64_t rows, int64_t vocab,
@@ -981,12 +983,13 @@ rescale_kernel(T* __restrict__ dlogits, RowGrid dg, RowDiv index, int64_t rows, 
       float x[V];
       unpack<T>(*at, x);
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] *= f;
+      for (int e = 0; e < V; ++e) x[e] = rescaled(x[e], f);
       *at = pack<T>(x);
     }
-    if ((int)threadIdx.x < head) row[threadIdx.x] = from_float<T>(to_float(row[threadIdx.x]) * f);
+    if ((int)threadIdx.x < head)
+      row[threadIdx.x] = from_float<T>(rescaled(to_float(row[threadIdx.x]), f));
     for (int64_t c = head + nvec * V + threadIdx.x; c < vocab; c += kThreads)
-      row[c] = from_float<T>(to_float(row[c]) * f);
+      row[c] = from_float<T>(rescaled(to_float(row[c]), f));
   }
 }
 

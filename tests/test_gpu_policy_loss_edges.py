@@ -209,3 +209,16 @@ def test_a_forward_and_backward_that_are_captured_together_can_be_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("up", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("vocab", [37, 1003, 1024])
+def test_ignored_rows_stay_zero_under_a_gradient_that_is_not_finite(vocab, up):
+    x, t, old, ref, adv = _inputs((2, 5, vocab), torch.bfloat16)
+    leaf = x.detach().requires_grad_()
+    loss, _ = kernels.policy_loss(leaf, t, old, adv, reference_log_probs=ref, kl_coef=0.1)
+    grads = [torch.autograd.grad(loss, leaf, torch.tensor(up, device=gu.DEV),
+                                 retain_graph=True)[0] for _ in range(2)]
+    for dx in grads:  # formed in the forward's pass, and in backward
+        assert (dx[t == IGNORE] == 0).all()
+        assert not torch.isfinite(dx[t != IGNORE]).any()
