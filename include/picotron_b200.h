@@ -464,7 +464,8 @@ PT_API int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, 
  * instead of twice. stats and coef are written as well (coef without the factor). dlogits as in
  * pt_token_logps_bwd. Rows of more than 1.5 MiB, or more than 2^28 rows, are refused:
  * pt_policy_loss_grad_supported says so beforehand. A bounded wait that runs out sets the device
- * error word (code 1). */
+ * error word (code 1) and makes what hangs on it NaN: the row's gradient, and with it the loss, or
+ * the part of the row's gradient that waited for the other parts' sums. */
 PT_API int pt_policy_loss_grad_supported(int64_t vocab, int64_t outer, int64_t inner, int dtype,
                                          int* supported);
 PT_API int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
@@ -480,6 +481,11 @@ PT_API int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer,
                                float* logps, float* stats, float* coef, void* dlogits,
                                int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
                                void* workspace, int64_t workspace_size, int dtype, void* stream);
+
+/* Self-test of that path without a GPU fault: the calling thread's next pt_policy_loss_grad gives
+ * each of its waits limit_cycles SM cycles (0 .. 2e9) instead of about a second, or gives them up
+ * without waiting (-1). Calls after that one wait as ever. No reference counterpart. */
+PT_API int pt_selftest_policy_wait(int64_t limit_cycles);
 
 /* Multiplies a gradient that was formed for the factor `expected` (finite, not 0) by *grad /
  * expected, in place; *grad is one fp32 value in device memory, and where it equals expected

@@ -147,6 +147,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                         _c_float, _c_ptr]),
     "pt_take_device_error": (_c_int, [ctypes.POINTER(_c_int)]),
     "pt_selftest_wait_timeout": (_c_int, [_c_i64, _c_ptr]),
+    "pt_selftest_policy_wait": (_c_int, [_c_i64]),
     "pt_swiglu_fwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
     "pt_swiglu_bwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
     "pt_rope_fwd": (_c_int, [_c_ptr, _c_i64_4, _c_ptr, _c_i64_4, _c_i64_4, _c_ptr, _c_ptr,
@@ -620,6 +621,12 @@ def selftest_wait_timeout(limit_cycles: int, stream: int) -> None:
 
     _check("pt_selftest_wait_timeout",
            library().pt_selftest_wait_timeout(limit_cycles, stream), None)
+
+
+def selftest_policy_wait(limit_cycles: int) -> None:
+    """The bounded waits of this thread's next policy_loss_grad (see pt_selftest_policy_wait)."""
+
+    _check("pt_selftest_policy_wait", library().pt_selftest_policy_wait(limit_cycles), None)
 
 
 def take_device_error() -> int:

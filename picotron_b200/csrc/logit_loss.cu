@@ -747,7 +747,7 @@ __device__ __forceinline__ void store_in_cluster(Stat* p, uint64_t* bar, uint32_
       : "memory");
 }
 // mbar_wait_bounded for data that other CTAs of the cluster have stored.
-__device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar) {
+__device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar, long long limit) {
   const long long t0 = clock64();
   for (;;) {
     uint32_t done;
@@ -759,14 +759,17 @@ __device__ __forceinline__ bool cluster_wait_bounded(uint64_t* bar) {
         : "r"(smem_addr(bar))
         : "memory");
     if (done) return true;
-    if (clock64() - t0 > kWaitLimitCycles) return false;
+    if (clock64() - t0 > limit) return false;
   }
 }
 
+// A wait that gives up (after wait_limit cycles; at once if that is negative) sets the error word
+// and makes the row NaN through its sum, whatever the slice then holds. What it waited for gets
+// the full time once more: it must not reach shared memory that another CTA has by then.
 template <typename T>
 __global__ void __launch_bounds__(kFusedThreads, kFusedBlocks)
 policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t vocab,
-                   int log2_cluster, PolicyTerms p, float grad, RowOut out,
+                   int log2_cluster, PolicyTerms p, float grad, long long wait_limit, RowOut out,
                    T* __restrict__ dlogits, RowGrid dg) {
   constexpr int V = Vec16<T>::N;
   const int cluster = 1 << log2_cluster;
@@ -838,10 +841,14 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
   Running acc;
   if (edge >= 0) acc.add1(xe);
   __syncwarp();
-  if (w1 > w0 && !mbar_wait_bounded(&bar[warp], 0) && lane == 0)
-    atomicExch(&g_logit_loss_error, kErrWait);
-  // Two vectors a trip: their loads and exponentials overlap.
   int v = w0 + lane;
+  if (w1 > w0 && (wait_limit < 0 || !mbar_wait_bounded(&bar[warp], 0, wait_limit))) {
+    if (lane == 0) atomicExch(&g_logit_loss_error, kErrWait);
+    mbar_wait_bounded(&bar[warp], 0);
+    acc.s.x = NAN;
+    v = w1;  // nothing is summed
+  }
+  // Two vectors a trip: their loads and exponentials overlap.
   for (; v + 32 < w1; v += 64) {
     float x[2 * V];
     unpack<T>(lds128(slice + (size_t)v * 16), x);
@@ -862,8 +869,12 @@ policy_grad_kernel(const T* __restrict__ logits, RowGrid lg, Targets tg, int64_t
   if (tid == 0) {
     if (cluster > 1) {
       // All CTAs' stores have arrived after this: none reaches into a CTA that has ended.
-      if (!cluster_wait_bounded(&peer_bar)) atomicExch(&g_logit_loss_error, kErrWait);
       total = Stat{-INFINITY, 0.0f};
+      if (wait_limit < 0 || !cluster_wait_bounded(&peer_bar, wait_limit)) {
+        atomicExch(&g_logit_loss_error, kErrWait);
+        cluster_wait_bounded(&peer_bar, kWaitLimitCycles);
+        total.s = NAN;
+      }
       for (int c = 0; c < cluster; ++c) total.m = fmaxf(total.m, peer[c].m);
       for (int c = 0; c < cluster; ++c) total.s += sum_at(peer[c], total.m);
     }
@@ -1215,10 +1226,13 @@ void launch_grad(const Rows& g, const void* logits, const float2* stats, const f
       x, g.lg, g.tg, g.rows, g.vocab, splits, stats, coef, cg, grad, dx, dg);
 }
 
+// How long the next one-pass call of this thread waits (see pt_selftest_policy_wait).
+thread_local long long g_next_wait_limit = kWaitLimitCycles;
+
 template <typename T>
 int launch_policy_grad(const Rows& g, const void* logits, int cluster, const PolicyTerms& p,
-                       float grad, const RowOut& out, void* dlogits, const RowGrid& dg,
-                       cudaStream_t s) {
+                       float grad, long long wait_limit, const RowOut& out, void* dlogits,
+                       const RowGrid& dg, cudaStream_t s) {
   if (short_rows(g, sizeof(T), kShortVecs)) {
     policy_short_kernel<T><<<short_grid(g), kShortWarps * 32, 0, s>>>(
         static_cast<const T*>(logits), g.lg, g.tg, g.rows, g.vocab, p, grad, out,
@@ -1248,7 +1262,8 @@ int launch_policy_grad(const Rows& g, const void* logits, int cluster, const Pol
     int log2_cluster = 0;
     while (1 << log2_cluster < cluster) ++log2_cluster;
     e = cudaLaunchKernelEx(&cfg, policy_grad_kernel<T>, static_cast<const T*>(logits), g.lg, g.tg,
-                           g.vocab, log2_cluster, p, grad, out, static_cast<T*>(dlogits), dg);
+                           g.vocab, log2_cluster, p, grad, wait_limit, out, static_cast<T*>(dlogits),
+                           dg);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1442,6 +1457,8 @@ int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_
                         double grad, float* loss, float* logps, float* stats, float* coef,
                         void* dlogits, int64_t dlogits_outer_stride, int64_t dlogits_inner_stride,
                         void* workspace, int64_t workspace_size, int dtype, void* stream) {
+  const long long wait_limit = g_next_wait_limit;
+  g_next_wait_limit = kWaitLimitCycles;
   Rows g;
   Workspace w;
   PolicyTerms p;
@@ -1472,19 +1489,29 @@ int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_
     int st;
     switch (dtype) {
       case PT_FLOAT32:
-        st = launch_policy_grad<float>(g, logits, cluster, p, (float)grad, out, dlogits, dg, s);
+        st = launch_policy_grad<float>(g, logits, cluster, p, (float)grad, wait_limit, out,
+                                       dlogits, dg, s);
         break;
       case PT_FLOAT16:
-        st = launch_policy_grad<__half>(g, logits, cluster, p, (float)grad, out, dlogits, dg, s);
+        st = launch_policy_grad<__half>(g, logits, cluster, p, (float)grad, wait_limit, out,
+                                       dlogits, dg, s);
         break;
       default:
-        st = launch_policy_grad<__nv_bfloat16>(g, logits, cluster, p, (float)grad, out, dlogits,
-                                               dg, s);
+        st = launch_policy_grad<__nv_bfloat16>(g, logits, cluster, p, (float)grad, wait_limit, out,
+                                               dlogits, dg, s);
     }
     if (st) return st;
   }
   policy_sum_kernel<<<1, kSumThreads, 0, s>>>(w.term, g.rows, w.seq, sequences, loss);
   return check_launch("pt_policy_loss_grad");
+}
+
+int pt_selftest_policy_wait(int64_t limit_cycles) {
+  if (limit_cycles < -1 || limit_cycles > kWaitLimitCycles)
+    return set_error(PT_ERR_INVALID_ARGUMENT, "limit_cycles must be in [-1, %lld] (got %lld)",
+                     kWaitLimitCycles, (long long)limit_cycles);
+  g_next_wait_limit = limit_cycles;
+  return ok();
 }
 
 int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t inner,

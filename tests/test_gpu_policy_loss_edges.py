@@ -222,3 +222,30 @@ def test_ignored_rows_stay_zero_under_a_gradient_that_is_not_finite(vocab, up):
     for dx in grads:  # formed in the forward's pass, and in backward
         assert (dx[t == IGNORE] == 0).all()
         assert not torch.isfinite(dx[t != IGNORE]).any()
+
+
+@pytest.mark.parametrize("limit", [-1, 0])
+@pytest.mark.parametrize("path", PATHS)
+def test_waits_that_run_out_leave_nan_and_the_error_word(path, limit):
+    """Waits that are given up at once (-1), or after one look (0, which may see the data): what was
+    not waited for is NaN and said so; nothing of it reaches the next call."""
+
+    args = (*_inputs(*PATHS[path][:2]), 0.1, path)
+    want_loss, want_lp, want = _call(*args)
+    t = args[1]
+    _capi.selftest_policy_wait(limit)
+    loss, lp, dx = _call(*args)
+    code = _capi.take_device_error()
+    if path.startswith("one pass") and limit < 0:
+        assert code == 1 and torch.isnan(loss)
+        assert torch.isnan(dx[t != IGNORE]).all() and torch.isnan(lp[t != IGNORE]).all()
+    elif path.startswith("one pass") and code:
+        assert code == 1 and (torch.isnan(dx) | (dx == want)).all()
+    else:
+        assert code == 0 and torch.equal(loss, want_loss) and torch.equal(lp, want_lp)
+        assert dx is None or torch.equal(dx, want)
+    assert dx is None or (dx[t == IGNORE] == 0).all()
+    _capi.selftest_policy_wait(2_000_000_000)
+    loss, lp, dx = _call(*args)
+    assert torch.equal(loss, want_loss) and (dx is None or torch.equal(dx, want))
+    assert _capi.take_device_error() == 0
