@@ -520,9 +520,11 @@ PT_API int pt_adamw_step(float* const* params, const float* const* grads,
  * v = b2 v + (1 - b2) (g g) with each product and sum rounded to fp32, new scales max|m| / 127^2
  * and max v / 255^4 of the block (0 where that is below the smallest normal number), new codes
  * the nearest ones in the square-root / fourth-root domain (ties to even), at least 1 where
- * v > 0. Code arrays have numels[i] elements, scale arrays ceil(numels[i] / 256); zeros are the
- * state before the first step. The parameters must not overlap one another. A non-finite
- * gradient makes the moments of its whole block non-finite. No reference counterpart (its
+ * v > 0 and the scale is. Code arrays have numels[i] elements, scale arrays ceil(numels[i] / 256);
+ * zeros are the state before the first step. The parameters must not overlap one another. eps must
+ * be at least 1e-12: a block whose largest v is below 5e-29 has a scale of 0 and leaves eps alone in
+ * the next denominator. A non-finite gradient makes the moments of its whole block non-finite, and
+ * one whose square is (beyond 1.8e19) exp_avg_sq of its block. No reference counterpart (its
  * optimizer is torch.optim.AdamW, src/picotron/training/train_loop.py:302-325). */
 PT_API int pt_adamw8_step(void* const* params, const void* const* grads,
                           int8_t* const* exp_avg_codes, float* const* exp_avg_scales,

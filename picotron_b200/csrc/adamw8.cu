@@ -5,8 +5,8 @@
 //   exp_avg_sq = c^4 s     with c in [0, 255]    and s = max exp_avg_sq / 255^4,
 // so codes are uniform in the square root of exp_avg and in the fourth root of exp_avg_sq (the
 // square root of the update's denominator): small values keep a relative step that grows only
-// with the root of their distance to the block's largest. A positive exp_avg_sq never takes code
-// 0, which would drop the denominator to eps. The step itself is AdamW in fp32:
+// with the root of their distance to the block's largest. A positive exp_avg_sq under a positive
+// scale never takes code 0, which would drop the denominator to eps. The step itself is AdamW in fp32:
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g g       (every product and sum rounded)
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Each new code is the one nearest to the new fp32 moment in the root's domain. The candidate
@@ -41,6 +41,12 @@ constexpr float kTiny = 1.17549435e-38f;  // smallest normal: a smaller scale is
 constexpr float kMomentScale = (float)(1.0 / 16129.0);        // 127^-2
 constexpr float kSquareScale = (float)(1.0 / 4228250625.0);   // 255^-4
 constexpr float kBorder = 0.4999f;
+// A block whose largest exp_avg_sq is below 255^4 kTiny = 5e-29 keeps a scale of 0, and eps alone
+// is left in the next step's denominator. Its gradients were below sqrt(5e-29 / (1 - b2)), and so
+// is m / (1 - b1^t): with an eps of 1e-12 a step is at most 0.22 lr for a b2 of 0.999 (0.7 lr for
+// 0.9999). An eps of 1e-15 would let it be 220 lr, and one below kTiny, which the approximate
+// square root and reciprocal take for 0, infinite.
+constexpr double kLeastEps = 1e-12;
 
 
 struct Tensor {
@@ -533,8 +539,8 @@ int pt_adamw8_step(void* const* params, const void* const* grads, int8_t* const*
   if (!params || !grads || !exp_avg_codes || !exp_avg_scales || !exp_avg_sq_codes ||
       !exp_avg_sq_scales || !numels || !steps || !lrs || !weight_decays)
     return set_error(PT_ERR_INVALID_ARGUMENT, "a tensor list pointer is NULL");
-  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
-    return set_error(PT_ERR_INVALID_ARGUMENT, "betas must be in [0, 1) and eps >= 0");
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= kLeastEps))
+    return set_error(PT_ERR_INVALID_ARGUMENT, "betas must be in [0, 1) and eps >= 1e-12");
   // Everything is checked before the first launch: a refused call changes nothing.
   for (int i = 0; i < num_tensors; ++i) {
     if (int st = check_state(i, numels[i], exp_avg_codes[i], exp_avg_scales[i],

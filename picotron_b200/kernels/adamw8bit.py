@@ -22,6 +22,7 @@ from picotron_b200 import _capi, ops
 from picotron_b200.errors import TritonAdamWUnavailable
 
 BLOCK = 256  # elements that share a scale
+LEAST_EPS = 1e-12  # what a block's exp_avg_sq may be dropped next to (see pt_adamw8_step)
 _STATE = {"exp_avg_codes": torch.int8, "exp_avg_scales": torch.float32,
           "exp_avg_sq_codes": torch.uint8, "exp_avg_sq_scales": torch.float32}
 
@@ -84,6 +85,9 @@ def adamw8bit_step(params: Sequence[Tensor], grads: Sequence[Tensor],
     [ceil(n / 256)], ``exp_avg_sq_codes`` uint8 [n] and ``exp_avg_sq_scales`` float32 [ceil(n /
     256)] (any shape with that many elements; zeros before the first step). ``step`` counts this
     step (1 for the first); ``step``, ``lr`` and ``weight_decay`` are one value or one per tensor.
+    ``eps`` is at least 1e-12: squares below 5e-29 are not kept, which leaves ``eps`` alone in the
+    denominator. A gradient that is not finite, or whose square is not (beyond 1.8e19), spoils the
+    moments of its block of 256.
     Nothing is changed when the call is refused. The step's scalars are host values, so a captured
     CUDA graph would replay the same step count.
     """
@@ -147,15 +151,17 @@ class AdamW8bit(Optimizer):
     """AdamW whose moments are held in 8 bits (see the module's description).
 
     Parameters: dense contiguous CUDA tensors in float32, float16 or bfloat16, updated in their
-    own dtype (no separate master copy). Arguments as torch.optim.AdamW's; amsgrad is not
-    offered. ``state_dict`` holds the codes and scales; ``load_state_dict`` keeps their dtypes.
+    own dtype (no separate master copy). Arguments as torch.optim.AdamW's, with ``eps`` at least
+    1e-12; amsgrad is not offered. ``state_dict`` holds the codes and scales; ``load_state_dict`` keeps their dtypes.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.01, *,
                  maximize: bool = False) -> None:
-        if lr < 0 or eps < 0 or weight_decay < 0:
-            raise ValueError("lr, eps and weight_decay must be >= 0")
+        if lr < 0 or weight_decay < 0:
+            raise ValueError("lr and weight_decay must be >= 0")
+        if not eps >= LEAST_EPS:
+            raise ValueError(f"eps must be at least {LEAST_EPS}: {eps}")
         if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError(f"betas must be in [0, 1): {betas}")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,

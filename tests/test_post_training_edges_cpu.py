@@ -3,9 +3,14 @@ test_post_training_cpu.py."""
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import pytest
+import torch
 
 from picotron_b200 import _capi
+from picotron_b200.kernels import AdamW8bit
 
 
 def test_wait_limits_of_the_self_test_are_checked():
@@ -13,3 +18,23 @@ def test_wait_limits_of_the_self_test_are_checked():
         with pytest.raises(_capi.PtError, match="limit_cycles"):
             _capi.selftest_policy_wait(limit)
     _capi.selftest_policy_wait(2_000_000_000)  # as without it
+
+
+def test_an_eps_below_what_the_states_can_drop_is_refused():
+    """Blocks whose largest exp_avg_sq is below 255^4 times the smallest normal number keep none of
+    it, so that eps alone is left in the denominator of the next step."""
+
+    p = torch.nn.Parameter(torch.zeros(4))
+    for eps in (0.0, 1e-45, 1e-30, 1e-13):
+        with pytest.raises(ValueError, match="eps"):
+            AdamW8bit([p], eps=eps)
+    AdamW8bit([p], eps=1e-12)
+    lib = _capi.library()
+    one = (ctypes.c_void_p * 1)(None)
+    n, step = (ctypes.c_int64 * 1)(0), (ctypes.c_int64 * 1)(1)
+    lr = (ctypes.c_double * 1)(0.1)
+    for eps, want in ((0.0, _capi.PT_ERR_INVALID_ARGUMENT), (1e-13, _capi.PT_ERR_INVALID_ARGUMENT),
+                      (math.nan, _capi.PT_ERR_INVALID_ARGUMENT)):
+        assert lib.pt_adamw8_step(one, one, one, one, one, one, n, step, lr, lr, 1, 0.9, 0.99, eps, 0,
+                                  0, None) == want
+        assert "eps" in _capi.last_error()
