@@ -37,6 +37,7 @@ import functools
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from picotron_b200 import _capi
 from picotron_b200.errors import (
@@ -695,6 +696,9 @@ class _Op:
             _LIBRARY.impl(name, self._autograd, "Autograd")
 
     def _autograd(self, *args):
+        # Inside a forward-mode level a tensor may carry a tangent, which apply refuses.
+        if forward_ad._current_level >= 0:
+            return self.function.apply(*args)
         if torch.is_grad_enabled():
             for a in args:
                 if isinstance(a, Tensor) and a.requires_grad:
