@@ -92,12 +92,26 @@ def adamw8bit_step(params: Sequence[Tensor], grads: Sequence[Tensor],
     CUDA graph would replay the same step count.
     """
 
+    _checked_step(params, grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes,
+                  exp_avg_sq_scales, step, lr, beta1, beta2, eps, weight_decay, maximize)()
+
+
+def _checked_step(params, grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes,
+                  exp_avg_sq_scales, step, lr, beta1, beta2, eps, weight_decay, maximize):
+    """adamw8bit_step's checks; returns the step itself, to be called under no_grad."""
+
     count = len(params)
     if count == 0 and not any(map(len, (grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes,
                                         exp_avg_sq_scales))):
-        return
+        return lambda: None
     if count == 0:
         raise TritonAdamWUnavailable("all tensor lists must have the same length.")
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= LEAST_EPS):
+        raise TritonAdamWUnavailable(f"betas must be in [0, 1) and eps at least {LEAST_EPS}.")
+    steps = _per_tensor(step, count, "step")
+    if min(steps) < 1:
+        raise TritonAdamWUnavailable("step counts the step that is taken: at least 1.")
+    lrs, decays = _per_tensor(lr, count, "lr"), _per_tensor(weight_decay, count, "weight_decay")
     first = params[0]
     ops.check_device(first.device, TritonAdamWUnavailable)
     code = ops._dtype_code(first, TritonAdamWUnavailable)
@@ -113,13 +127,16 @@ def adamw8bit_step(params: Sequence[Tensor], grads: Sequence[Tensor],
     _refuse_shared("parameters", at_params, sizes, first.element_size())
     for name, at, width in zip(_STATE, at_states, (1, 4, 1, 4)):
         _refuse_shared(name, at, scales if width == 4 else sizes, width)
-    with ops._OnDevice(first.device):
-        _capi.adamw8_step(at_params, at_grads, *at_states, sizes,
-                          _per_tensor(step, count, "step"), _per_tensor(lr, count, "lr"),
-                          _per_tensor(weight_decay, count, "weight_decay"), beta1, beta2, eps,
-                          maximize, code, ops._raw_stream(first.device), TritonAdamWUnavailable)
-    # As an in-place torch operation does: a backward that saved a parameter notices.
-    torch.autograd.graph.increment_version(params)
+
+    def run() -> None:
+        with ops._OnDevice(first.device):
+            _capi.adamw8_step(at_params, at_grads, *at_states, sizes, steps, lrs, decays, beta1,
+                              beta2, eps, maximize, code, ops._raw_stream(first.device),
+                              TritonAdamWUnavailable)
+        # As an in-place torch operation does: a backward that saved a parameter notices.
+        torch.autograd.graph.increment_version(params)
+
+    return run
 
 
 @torch.no_grad()
@@ -192,16 +209,17 @@ class AdamW8bit(Optimizer):
                 if p.grad.is_sparse or not p.is_cuda:
                     raise TritonAdamWUnavailable("AdamW8bit takes dense CUDA parameters.")
                 calls[(p.device, p.dtype, *key)].append((p, group))
+        steps = []  # all checked before the first is taken: a refused step changes nothing
         for (_, _, beta1, beta2, eps, maximize), items in calls.items():
             params = [p for p, _ in items]
             # Not self.state[p], which would leave an empty entry behind a refused step.
             states = [self.state.get(p) or self._new_state(p) for p in params]
-            adamw8bit_step(params, [p.grad for p in params],
-                           *([s[name] for s in states] for name in _STATE),
-                           step=[s["step"] + 1 for s in states],
-                           lr=[float(g["lr"]) for _, g in items], beta1=beta1, beta2=beta2,
-                           eps=eps, weight_decay=[float(g["weight_decay"]) for _, g in items],
-                           maximize=maximize)
+            steps.append((params, states, _checked_step(
+                params, [p.grad for p in params], *([s[name] for s in states] for name in _STATE),
+                [s["step"] + 1 for s in states], [float(g["lr"]) for _, g in items], beta1, beta2,
+                eps, [float(g["weight_decay"]) for _, g in items], maximize)))
+        for params, states, run in steps:
+            run()
             for p, s in zip(params, states):
                 s["step"] += 1
                 self.state[p] = s

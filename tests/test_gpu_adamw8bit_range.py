@@ -1,4 +1,4 @@
-"""The 8-bit AdamW step at the ends of what its states can hold."""
+"""The 8-bit AdamW step at the ends of what its states can hold, and what a refused one leaves."""
 
 from __future__ import annotations
 
@@ -7,7 +7,7 @@ import torch
 
 import gpu_utils as gu
 from picotron_b200.errors import TritonAdamWUnavailable
-from picotron_b200.kernels import adamw8bit_moments, adamw8bit_step
+from picotron_b200.kernels import AdamW8bit, adamw8bit_moments, adamw8bit_step
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,32 @@ def test_squares_beyond_the_range_count_as_not_finite():
     assert torch.isnan(v[0][256:512]).all() and torch.isfinite(m[0]).all()
     for s in (slice(0, 256), slice(512, 1000)):
         assert torch.equal(p[s], q[s]) and torch.isfinite(v[0][s]).all()
+
+
+def test_a_step_that_is_refused_for_one_group_takes_none():
+    """Groups of other betas or types are launches of their own; all are checked before the first."""
+
+    good = [torch.nn.Parameter(gu.randn((40, 3), 1)), torch.nn.Parameter(gu.randn((9,), 2))]
+    bad = torch.nn.Parameter(gu.randn((6, 4), 3).t())
+    opt = AdamW8bit([{"params": good}, {"params": [bad], "betas": (0.8, 0.9)}])
+    for p in (*good, bad):
+        p.grad = torch.ones_like(p)
+    before = [p.detach().clone() for p in (*good, bad)]
+    with pytest.raises(TritonAdamWUnavailable):
+        opt.step()
+    assert len(opt.state) == 0
+    assert all(torch.equal(p, b) for p, b in zip((*good, bad), before))
+    bad.grad = None
+    opt.step()
+    assert [opt.state[p]["step"] for p in good] == [1, 1] and len(opt.state) == 2
+    bad.grad = torch.ones_like(bad)
+    before = [p.detach().clone() for p in good]
+    with pytest.raises(TritonAdamWUnavailable):
+        opt.step()
+    assert [opt.state[p]["step"] for p in good] == [1, 1]
+    assert all(torch.equal(p, b) for p, b in zip(good, before))
+    bad.grad = None
+    opt.param_groups[0]["eps"] = 0.0  # may be set, or loaded, after construction
+    with pytest.raises(TritonAdamWUnavailable, match="eps"):
+        opt.step()
+    assert all(torch.equal(p, b) for p, b in zip(good, before))
