@@ -398,8 +398,9 @@ PT_API int pt_cross_entropy_bwd(const void* logits, int64_t vocab, int64_t outer
 PT_API int pt_logit_loss_workspace(int64_t vocab, int64_t outer, int64_t inner, int dtype,
                                    int64_t* bytes);
 
-/* logps[r] = x_r[target] - log(sum(exp(x_r))) (dense [rows]) and stats[r] = (max(x_r), 1 /
- * sum(exp(x_r - max))) (dense [rows, 2]), which the backward reads. */
+/* logps[r] = x_r[target] - log(sum(exp(x_r))) (dense [rows]) and stats[r] = (m, 1 / sum(exp(x_r -
+ * m))) (dense [rows, 2], 8-byte aligned), which the backward reads: m is a value from max(x_r) to
+ * max(x_r) + 9, not the maximum itself; (0, 0) where there is no target. */
 PT_API int pt_token_logps_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t inner,
                               int64_t logits_outer_stride, int64_t logits_inner_stride,
                               const int64_t* targets, int64_t targets_outer_stride,

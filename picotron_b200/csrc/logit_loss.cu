@@ -1064,6 +1064,15 @@ int check_optional(const void* p, const char* name, int64_t rows) {
   return rows > 0 ? check_device_ptr(p, name) : PT_OK;
 }
 
+// stats [rows, 2], read and written as pairs.
+int check_stats(const float* stats, int64_t rows) {
+  if (rows == 0) return PT_OK;
+  if (int st = check_device_ptr(stats, "stats")) return st;
+  if (reinterpret_cast<uintptr_t>(stats) % 8)
+    return set_error(PT_ERR_INVALID_ARGUMENT, "stats must be 8-byte aligned");
+  return PT_OK;
+}
+
 struct Workspace {
   double* logps;
   double* term;
@@ -1169,7 +1178,7 @@ int check_policy(Rows& g, Workspace& w, PolicyTerms& p, const PolicyInputs& in,
   if (in.ref)
     if (int st = check_optional(in.ref, "reference", g.rows)) return st;
   if (int st = check_optional(logps, "logps", g.rows)) return st;
-  if (int st = check_optional(stats, "stats", g.rows)) return st;
+  if (int st = check_stats(stats, g.rows)) return st;
   if (int st = check_optional(coef, "coef", g.rows)) return st;
   if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
   p.old = in.old;
@@ -1320,7 +1329,7 @@ int pt_token_logps_fwd(const void* logits, int64_t vocab, int64_t outer, int64_t
                           targets_inner_stride, ignore_index, dtype))
     return st;
   if (int st = check_optional(logps, "logps", g.rows)) return st;
-  if (int st = check_optional(stats, "stats", g.rows)) return st;
+  if (int st = check_stats(stats, g.rows)) return st;
   Workspace w;
   if (int st = take_workspace(w, g, workspace, workspace_size)) return st;
   row_stats(g, logits, dtype, w.part, RowOut{reinterpret_cast<float2*>(stats), logps, nullptr},
@@ -1341,7 +1350,7 @@ int pt_token_logps_bwd(const void* logits, int64_t vocab, int64_t outer, int64_t
                           targets_inner_stride, ignore_index, dtype))
     return st;
   if (g.rows == 0) return ok();
-  if (int st = check_device_ptr(stats, "stats")) return st;
+  if (int st = check_stats(stats, g.rows)) return st;
   if (int st = check_device_ptr(coef, "coef")) return st;
   if (int st = check_device_ptr(dlogits, "dlogits")) return st;
   if (grad)
@@ -1382,7 +1391,7 @@ int pt_preference_loss_fwd(const void* logits, int64_t vocab, int64_t outer, int
     return st;
   if (int st = check_device_ptr(loss, "loss")) return st;
   if (int st = check_optional(reference, "reference", g.rows)) return st;
-  if (int st = check_optional(stats, "stats", g.rows)) return st;
+  if (int st = check_stats(stats, g.rows)) return st;
   if (int st = check_optional(rewards, "rewards", outer)) return st;
   if (int st = check_optional(coef, "coef", outer)) return st;
   Workspace w;

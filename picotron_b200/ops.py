@@ -873,8 +873,11 @@ def _logit_loss_backward(logits: Tensor, targets: Tensor, stats: Tensor, coef: T
     (and any strides), grad is one value."""
 
     _ll_inputs(logits, targets, (coef,))
-    if stats.shape != (*targets.shape, 2) or not stats.is_contiguous():
+    if (stats.shape != (*targets.shape, 2) or not stats.is_contiguous()
+            or stats.dtype != torch.float32 or stats.device != logits.device):
         raise TritonLogitLossUnavailable("stats must be the forward's.")
+    if grad is not None and (grad.numel() != 1 or grad.device != logits.device):
+        raise TritonLogitLossUnavailable("grad must be one value on the logits' device.")
     return _ll_backward(logits, targets, stats, coef, grad, ignore_index)
 
 
