@@ -60,15 +60,16 @@ def _per_tensor(value, count: int, name: str) -> list:
     return [value] * count
 
 
-def _refuse_shared(name: str, addresses: Sequence[int], sizes: Sequence[int], width: int) -> None:
-    """Two entries over the same memory would be updated by two blocks at once."""
+def _refuse_shared(spans: list[tuple[int, int]]) -> None:
+    """(address, bytes) of all that a step writes. Memory that two entries share, of one list or of
+    two, would be updated twice at once."""
 
     end = 0
-    for at, n in sorted(zip(addresses, sizes)):
-        if n:
-            if at < end:
-                raise TritonAdamWUnavailable(f"two of the {name} share memory.")
-            end = at + n * width
+    for at, size in sorted(spans):
+        if at < end and size:
+            raise TritonAdamWUnavailable("two of the parameters and states share memory.")
+        if size:
+            end = at + size
 
 
 @torch.no_grad()
@@ -124,9 +125,10 @@ def _checked_step(params, grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes
             raise TritonAdamWUnavailable("parameters and gradients must have the same shapes.")
     at_states, scales = _state_addresses(
         (exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales), sizes, device)
-    _refuse_shared("parameters", at_params, sizes, first.element_size())
-    for name, at, width in zip(_STATE, at_states, (1, 4, 1, 4)):
-        _refuse_shared(name, at, scales if width == 4 else sizes, width)
+    width = first.element_size()
+    extents = ([n * width for n in sizes], sizes, [4 * n for n in scales])
+    _refuse_shared([span for at, which in zip((at_params, *at_states), (0, 1, 2, 1, 2))
+                    for span in zip(at, extents[which])])
 
     def run() -> None:
         with ops._OnDevice(first.device):

@@ -102,3 +102,18 @@ def test_a_step_that_is_refused_for_one_group_takes_none():
     with pytest.raises(TritonAdamWUnavailable, match="eps"):
         opt.step()
     assert all(torch.equal(p, b) for p, b in zip(good, before))
+
+
+def test_states_that_share_memory_across_lists_are_refused():
+    p, g, state = _fresh(600, 31)
+    mc, ms, vc, vs = state
+    flat = torch.zeros(5000, dtype=torch.uint8, device=gu.DEV)
+    inside = flat[:2400].view(torch.float32)  # a parameter of 600 elements over its own codes
+    for params, held in ((p, [mc, ms, mc.view(torch.uint8), vs]), (p, [mc, ms, vc, ms]),
+                         (inside, [flat[2399:2999].view(torch.int8), ms, vc, vs]),
+                         (p, [mc, flat[1000:1012].view(torch.float32), flat[411:1011], vs])):
+        before = [t.clone() for t in (params, *held)]
+        with pytest.raises(TritonAdamWUnavailable, match="share memory"):
+            _call(params, g, held, 1)
+        assert all(torch.equal(a, b) for a, b in zip((params, *held), before))
+    _call(inside, g, [flat[2400:3000].view(torch.int8), ms, vc, vs], 1)  # next to one another
