@@ -6,7 +6,8 @@
 // so codes are uniform in the square root of exp_avg and in the fourth root of exp_avg_sq (the
 // square root of the update's denominator): small values keep a relative step that grows only
 // with the root of their distance to the block's largest. A positive exp_avg_sq under a positive
-// scale never takes code 0, which would drop the denominator to eps. The step itself is AdamW in fp32:
+// scale never takes code 0, which would drop the denominator to eps. The step itself is AdamW in
+// fp32:
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g g       (every product and sum rounded)
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 // Each new code is the one nearest to the new fp32 moment in the root's domain. The candidate
@@ -17,8 +18,12 @@
 // does not depend on how the root was computed.
 //
 // One warp per block of 256, eight elements per lane; the block's two maxima by integer max over
-// the warp (for values >= 0 the bit patterns order like the values, NaN above all). Bytes per element: 3 parameter widths (parameter read and written, gradient read) + 4;
-// the kernel is bound by HBM.
+// the warp (for values >= 0 the bit patterns order like the values, NaN above all). The parameter's
+// update alone takes the approximate square root and reciprocal (2^-23 each): it is within 2^-21
+// of its value, less than the rounding of an fp32 parameter of eight times its size or more.
+// Bytes per element: 3 parameter widths (parameter read and written, gradient read) + 4. In fp32
+// the kernel is bound by HBM (436 M parameters: 1.07 ms, the copy rate); in 16 bits, with 10 bytes
+// an element in place of 16 and the same arithmetic, by instruction issue (0.87 ms, 0.77 of it).
 #include <algorithm>
 #include <cmath>
 

@@ -5,7 +5,9 @@
 //   a = positions[b, s] * inv_freq[i],
 // formed in 64 bits and reduced to within half a turn there (a far position times a frequency
 // has lost its fraction in 32 bits: at position 10^6 the product is off by 0.03 radian), so one
-// single-precision sincospi of the rest follows. c = scale cos a, s = scale sin a, and
+// single-precision sincospi of the rest follows: rounding the rest to fp32 moves it by at most
+// 2^-25 pi radian, less than the two products and the sum of an output are rounded by. With
+// c = scale cos a, s = scale sin a,
 //   out_1 = x_1 c - x_2 s,  out_2 = x_1 s + x_2 c
 // for the pairs (x[2i], x[2i+1]) (INTERLEAVED) or (x[i], x[i + R/2]) (ROTATE_HALF); x[R:] is
 // copied. The backward is the transpose, the same with s negated. Each output is rounded once.
@@ -22,7 +24,7 @@ namespace pt {
 namespace {
 
 // 128 threads (64 and 256 took 1.1 and 1.2 times as long at B 8, S 2048, 32 + 8 heads of 128,
-// bf16: 54 us, 0.95 of the HBM peak). Units in flight per thread: five where a token has that
+// bf16: 54 us, 0.95 of the copy rate). Units in flight per thread: five where a token has that
 // many, as there, else three (54 against 60 us there; 3.1 against 3.9 us for 32 decoded tokens).
 constexpr int kThreads = 128;
 constexpr int kManyUnits = 5;

@@ -215,7 +215,9 @@ class RotaryEmbedding(nn.Module):
     attributes may be set on the module: ``rotary_dim`` (only the first elements of each head are
     rotated) and ``scaling`` (frequencies for long contexts: a dict of the keywords of
     ``kernels.rotary_frequencies``, e.g. ``{"scaling": "yarn", "factor": 8.0,
-    "original_length": 4096}``).
+    "original_length": 4096}``). With either, or with positions, the first call of a setting
+    copies its frequencies to the device, which a CUDA graph under capture refuses: call the
+    module once before.
     """
 
     def __init__(

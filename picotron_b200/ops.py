@@ -660,9 +660,10 @@ cross_entropy.register_autograd(_ce_backward, setup_context=_ce_setup)
 
 # The ops below are registered through torch.library.Library with an autograd.Function each, where
 # those above use custom_op: the same torch.ops.picotron_b200 entries, fake implementations and
-# autograd, but small calls take the host's time, and a forward and backward through custom_op
-# spent 148 us there, one through Library and Function 42 (without kernels). Calls on plain
-# tensors outside of tracing and dispatch modes skip the dispatcher as well.
+# autograd, but small calls take the host's time. A forward and backward of an op that launches
+# nothing takes 97 us through custom_op, 58 through Library and Function and 61 in a bare Function
+# (B200 host). Calls on plain tensors outside of tracing and dispatch modes skip the dispatcher as
+# well. Forward-mode derivatives are refused.
 
 _LIBRARY = torch.library.Library("picotron_b200", "FRAGMENT")
 _PLAIN = (Tensor, torch.nn.Parameter)
