@@ -171,7 +171,8 @@ class AdamW8bit(Optimizer):
 
     Parameters: dense contiguous CUDA tensors in float32, float16 or bfloat16, updated in their
     own dtype (no separate master copy). Arguments as torch.optim.AdamW's, with ``eps`` at least
-    1e-12; amsgrad is not offered. ``state_dict`` holds the codes and scales; ``load_state_dict`` keeps their dtypes.
+    1e-12; amsgrad is not offered. ``state_dict`` holds the codes and scales; ``load_state_dict``
+    keeps their dtypes.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),

@@ -15,7 +15,8 @@ The logits gradient is the only one: per-token inputs and returned log-probabili
 of the losses carry none. Targets outside [0, V) give NaN and set the library's device error
 word (a kernel cannot raise); their logits get a gradient of zeros. NaN, and what has no value in
 64 bits either, in the logits or per-token inputs of a position with a target makes the loss and
-that position's gradient NaN (in the preference loss, its pair's). Calls that cannot run raise :class:`TritonLogitLossUnavailable`.
+that position's gradient NaN (in the preference loss, its pair's). Calls that cannot run raise
+:class:`TritonLogitLossUnavailable`.
 """
 
 from __future__ import annotations

@@ -195,7 +195,9 @@ def _kept(cache: dict[tuple, tuple], key: tuple, build) -> tuple:
     tensors that a CUDA graph under capture has yet to fill are returned but not kept."""
 
     held = cache.get(key)
-    if torch.compiler.is_compiling():  # what follows cannot be traced
+    # What follows cannot be traced: a compiled first call keeps what its own mode gives, which an
+    # eager call then replaces.
+    if torch.compiler.is_compiling():
         if held is None:
             held = cache[key] = build()
         return held
