@@ -460,7 +460,8 @@ PT_API int pt_policy_loss_fwd(const void* logits, int64_t vocab, int64_t outer, 
                               int dtype, void* stream);
 
 /* pt_policy_loss_fwd and, in the same pass over the logits, dlogits = grad * d loss / d logits,
- * for a caller that knows (or expects) the factor `grad` that the loss's gradient will have:
+ * for a caller that knows (or expects) the factor `grad`, finite in fp32, that the loss's gradient
+ * will have:
  * rows stay on chip between their statistics and their gradient, so the logits are read once
  * instead of twice. stats and coef are written as well (coef without the factor). dlogits as in
  * pt_token_logps_bwd. Rows of more than 1.5 MiB, or more than 2^28 rows, are refused:
@@ -488,7 +489,7 @@ PT_API int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer,
  * without waiting (-1). Calls after that one wait as ever. No reference counterpart. */
 PT_API int pt_selftest_policy_wait(int64_t limit_cycles);
 
-/* Multiplies a gradient that was formed for the factor `expected` (finite, not 0) by *grad /
+/* Multiplies a gradient that was formed for the factor `expected` (a normal fp32 number) by *grad /
  * expected, in place; *grad is one fp32 value in device memory, and where it equals expected
  * nothing is read or written. Zeros stay zeros, also where *grad is not finite. */
 PT_API int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t inner,

@@ -1472,6 +1472,8 @@ int pt_policy_loss_grad(const void* logits, int64_t vocab, int64_t outer, int64_
                         void* workspace, int64_t workspace_size, int dtype, void* stream) {
   const long long wait_limit = g_next_wait_limit;
   g_next_wait_limit = kWaitLimitCycles;
+  if (!std::isfinite((float)grad))
+    return set_error(PT_ERR_INVALID_ARGUMENT, "grad must be finite in fp32");
   Rows g;
   Workspace w;
   PolicyTerms p;
@@ -1534,8 +1536,9 @@ int pt_rescale_logits_grad(void* dlogits, int64_t vocab, int64_t outer, int64_t 
   if (int st = check_sizes(vocab, outer, inner, &rows)) return st;
   if (dtype_size(dtype) == 0)
     return set_error(PT_ERR_UNSUPPORTED_DTYPE, "unsupported dtype %d", dtype);
-  if (!std::isfinite(expected) || expected == 0.0)
-    return set_error(PT_ERR_INVALID_ARGUMENT, "expected must be finite and not 0");
+  // As fp32, which the gradient was formed with: a smaller factor has left nothing to rescale.
+  if (!std::isnormal((float)expected))
+    return set_error(PT_ERR_INVALID_ARGUMENT, "expected must be a normal fp32 number");
   if (rows == 0) return ok();
   if (int st = check_device_ptr(dlogits, "dlogits")) return st;
   if (int st = check_device_ptr(grad, "grad")) return st;

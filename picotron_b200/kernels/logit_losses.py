@@ -21,13 +21,14 @@ that position's gradient NaN (in the preference loss, its pair's). Calls that ca
 
 from __future__ import annotations
 
-import math
-
 import torch
 from torch import Tensor
 
 from picotron_b200 import ops
 from picotron_b200.errors import TritonLogitLossUnavailable
+
+
+_FP32 = torch.finfo(torch.float32)
 
 
 def _check_tensors(**tensors) -> None:
@@ -104,9 +105,10 @@ def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantag
     gradient that the loss is expected to receive; ``backward`` then only compares. That is 1 by
     default (``loss.backward()``); give ``expected_grad`` where the loss is scaled before it, e.g.
     ``1 / steps`` for ``(loss / steps).backward()`` or a loss scaler's scale. Any other gradient
-    is still right but costs a pass to rescale, and rounds the result once more. float16 logits
-    form their gradient in ``backward`` unless ``expected_grad`` is given, since it would
-    underflow without the loss scale.
+    is still right but costs a pass to rescale, and rounds the result once more: to the logits'
+    type's smallest steps at the expected factor, so a guess that is far too small loses what is
+    below them. float16 logits form their gradient in ``backward`` unless ``expected_grad`` is
+    given, since it would underflow without the loss scale.
     """
 
     _check_tensors(logits=logits, targets=targets, old_log_probs=old_log_probs,
@@ -114,8 +116,8 @@ def policy_loss(logits: Tensor, targets: Tensor, old_log_probs: Tensor, advantag
     if aggregate not in ("token", "sequence"):
         raise TritonLogitLossUnavailable(
             f'aggregate must be "token" or "sequence", not {aggregate!r}')
-    if expected_grad is not None and not (math.isfinite(expected_grad) and expected_grad != 0):
-        raise TritonLogitLossUnavailable("expected_grad must be finite and not 0.")
+    if expected_grad is not None and not _FP32.tiny <= abs(expected_grad) <= _FP32.max:
+        raise TritonLogitLossUnavailable("expected_grad must be finite and not 0 in float32.")
     reference = None
     if kl_coef != 0.0:
         if reference_log_probs is None:

@@ -15,6 +15,7 @@ import torch
 
 import gpu_utils as gu
 from picotron_b200 import _capi, kernels
+from picotron_b200.errors import TritonLogitLossUnavailable
 
 pytestmark = pytest.mark.gpu
 
@@ -249,3 +250,10 @@ def test_waits_that_run_out_leave_nan_and_the_error_word(path, limit):
     loss, lp, dx = _call(*args)
     assert torch.equal(loss, want_loss) and (dx is None or torch.equal(dx, want))
     assert _capi.take_device_error() == 0
+
+
+def test_expected_gradients_that_fp32_does_not_hold_are_refused():
+    x, t, old, _, adv = _inputs(*PATHS["one pass"][:2])
+    for expected in (1e-50, -1e-40, 1e39):
+        with pytest.raises(TritonLogitLossUnavailable, match="expected_grad"):
+            kernels.policy_loss(x, t, old, adv, expected_grad=expected)

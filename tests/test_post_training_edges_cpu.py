@@ -38,3 +38,19 @@ def test_an_eps_below_what_the_states_can_drop_is_refused():
         assert lib.pt_adamw8_step(one, one, one, one, one, one, n, step, lr, lr, 1, 0.9, 0.99, eps, 0,
                                   0, None) == want
         assert "eps" in _capi.last_error()
+
+
+def test_factors_that_fp32_does_not_hold_are_refused():
+    """A gradient formed with 1e-50 or 1e39 is 0 or infinite, and no rescaling brings it back."""
+
+    lib, arg = _capi.library(), _capi.PT_ERR_INVALID_ARGUMENT
+    for expected in (1e-50, -1e-40, 1e39, math.inf, math.nan, 0.0):
+        assert lib.pt_rescale_logits_grad(None, 8, 0, 1, 8, 8, None, expected, 2, None) == arg
+    for expected in (2.0 ** -126, -3e38):
+        assert lib.pt_rescale_logits_grad(None, 8, 0, 1, 8, 8, None, expected, 2, None) == _capi.PT_OK
+    rows = (None, 0, 0)
+    for grad in (1e39, math.inf, math.nan):
+        assert lib.pt_policy_loss_grad(None, 8, 2, 3, 24, 8, *rows, -100, *rows, *rows, *rows, 0.2, 0.2,
+                                       0.0, 0, grad, None, None, None, None, *rows, None, 0, 2,
+                                       None) == arg
+        assert "grad" in _capi.last_error()
