@@ -640,32 +640,23 @@ struct PolicyRow {
     ref = p.ref != nullptr ? p.ref[p.rg.offset(i)] : 0.0f;
     weight = p.weight[i.outer];
   }
-  // max(-A r, -A clip(r)) and its derivative to lp: -A r where the unclipped term is the larger
-  // one. NaN of any input is kept in both (fmax and fmin return their other operand, so comparisons
-  // that it fails choose here).
-  template <typename F>
-  static __device__ __forceinline__ void clip(F r, F a, F low, F high, double& value,
-                                              double& slope) {
-    const F clipped = r < low ? low : r > high ? high : r;
-    const F gain = -a * r, bounded = -a * clipped;
-    const bool beyond = a > F(0) ? r > high : r < low;
-    const F larger = gain <= bounded ? bounded : gain;
-    value = larger;
-    slope = larger != larger ? larger : beyond ? F(0) : gain;
-  }
-  // The clipped term of r = e^(lp - old) and kl (e^g - g - 1) of g = ref - lp, whose derivative is
-  // kl (1 - e^g). The differences are taken in 64 bits. Exponentials of up to kOrdinary are taken
-  // in 32 bits: expf is within 2^-22 and expm1f within 2^-22 |e^g - 1| there, which is what an
-  // error of 2^-22 in the log-probability makes of r and of the KL term. Larger arguments are taken
-  // in 64 bits, where e^89 and above are finite, so that a zero advantage weighs nothing.
+  // max(-A r, -A clip(r)) + kl (e^g - g - 1) with r = e^(lp - old), g = ref - lp, and its
+  // derivative to lp. The clipped term is the larger one where r is above the upper border for a
+  // positive A, below the lower one for a negative A: -A times that border, which has no slope;
+  // elsewhere it is -A r, its own derivative. That of the KL term is kl (1 - e^g). NaN of any
+  // input is kept in both (fmax and fmin would drop it). All is in 64 bits but for the
+  // exponentials of up to kOrdinary: expf is within 2^-22 and expm1f within 2^-22 |e^g - 1| there,
+  // which is what an error of 2^-22 in the log-probability makes of r and of the KL term. Larger
+  // arguments are taken in 64 bits, where e^89 and above are finite, so that a zero advantage
+  // weighs nothing.
   __device__ __forceinline__ void term(const PolicyTerms& p, double lp, double& term,
                                        float& coef) const {
-    const double d = lp - (double)old;
-    double value, slope;
-    if (fabs(d) <= kOrdinary)
-      clip(expf((float)d), adv, (float)p.low, (float)p.high, value, slope);
-    else
-      clip(far_exp(d), (double)adv, p.low, p.high, value, slope);
+    const double d = lp - (double)old, a = (double)adv;
+    const double r = fabs(d) <= kOrdinary ? (double)expf((float)d) : far_exp(d);
+    const double border = a > 0.0 ? p.high : p.low;
+    const bool beyond = a > 0.0 ? r > border : r < border;
+    double value = -a * (beyond ? border : r);
+    double slope = beyond && value == value ? 0.0 : value;
     if (p.ref != nullptr) {
       const double g = (double)ref - lp;
       const double eg = fabs(g) <= kOrdinary ? (double)expm1f((float)g) : far_exp(g) - 1.0;

@@ -257,3 +257,20 @@ def test_expected_gradients_that_fp32_does_not_hold_are_refused():
     for expected in (1e-50, -1e-40, 1e39):
         with pytest.raises(TritonLogitLossUnavailable, match="expected_grad"):
             kernels.policy_loss(x, t, old, adv, expected_grad=expected)
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_clipped_terms_are_rounded_once(path):
+    """Where every position is clipped the loss hangs on no log-probability, so that the one rounding
+    to fp32 (2^-24 relative) is all that may be off; the gradient is zero."""
+
+    x, t, _, _, _ = _inputs(*PATHS[path][:2])
+    lp, keep = kernels.token_log_probs(x, t), t != IGNORE
+    for seed in range(12):
+        adv = gu.randn(t.shape, seed)
+        old = lp - torch.sign(adv) * 0.6  # ratios of 1.8 and 0.55
+        loss, _, dx = _call(x, t, old, None, adv, 0.0, path)
+        border = torch.where(adv > 0, 1.0 + 0.2 * torch.ones_like(adv, dtype=torch.float64), 1.0 - 0.2)
+        want = -(adv.double() * border)[keep].mean().item()
+        assert abs(loss.item() - want) <= 1.001 * 2.0 ** -24 * abs(want)
+        assert dx is None or not dx.any()
